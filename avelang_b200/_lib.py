@@ -32,6 +32,12 @@ EXPORTS = (
     "ave_fp4_linear_decode", "ave_fp4_linear_decode_workspace_bytes", "ave_fp4_gemm_allgather_quantized",
 )
 
+# every symbol include/ave_dense.h declares
+DENSE_EXPORTS = (
+    "ave_int8_quantize", "ave_int8_gemm", "ave_int8_gemm_gated", "ave_bf16_gemm_gated", "ave_bf16_gated_backward",
+    "ave_bf16_gated_backward_workspace_bytes", "ave_bf16_gemm_backward",
+)
+
 
 def load() -> ctypes.CDLL:
     """Load the shared library (without touching any GPU)."""
@@ -93,6 +99,20 @@ def load() -> ctypes.CDLL:
         L.ave_fp4_gemm_allgather_quantized.restype = i32
         L.ave_fp4_gemm_allgather_quantized.argtypes = [vp, vp, vp, vp, vp, vp, i64, i64, i64, i32, i32, ctypes.POINTER(Epilogue), i64, i64,
                                                        ctypes.POINTER(vp), ctypes.POINTER(vp), i32, vp]
+        L.ave_int8_quantize.restype = i32
+        L.ave_int8_quantize.argtypes = [vp, i64, i64, i64, vp, i64, vp, vp]
+        L.ave_int8_gemm.restype = i32
+        L.ave_int8_gemm.argtypes = [vp, i64, vp, vp, i64, vp, vp, i32, vp, i64, i64, i64, i64, vp]
+        L.ave_int8_gemm_gated.restype = i32
+        L.ave_int8_gemm_gated.argtypes = [vp, i64, vp, vp, i64, vp, vp, i64, vp, i32, vp, i64, i64, i64, i64, vp]
+        L.ave_bf16_gemm_gated.restype = i32
+        L.ave_bf16_gemm_gated.argtypes = [vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i64, vp, i64, i64, i64, i64, vp]
+        L.ave_bf16_gated_backward_workspace_bytes.restype = i64
+        L.ave_bf16_gated_backward_workspace_bytes.argtypes = [i64, i64]
+        L.ave_bf16_gated_backward.restype = i32
+        L.ave_bf16_gated_backward.argtypes = [vp, i64] * 6 + [i32, vp, i64, vp, vp, i64, vp, i64, i64, i64, i64, vp]
+        L.ave_bf16_gemm_backward.restype = i32
+        L.ave_bf16_gemm_backward.argtypes = [vp, i64] * 5 + [i64, i64, i64, vp]
         L.ave_fp4_set_trace.restype = i32
         L.ave_fp4_set_trace.argtypes = [vp, i64]
         _lib = L

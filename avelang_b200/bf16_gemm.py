@@ -18,7 +18,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _dense, _lib
 from .fp4_gemm import GEMM_AUTO
 
 GROUP_K = 8
@@ -74,3 +74,34 @@ def gemm_pipeline_transposed_b(
         _lib.check(L.ave_bf16_gemm(ctypes.c_void_p(A.data_ptr()), ctypes.c_void_p(B.data_ptr()), ctypes.c_void_p(out.data_ptr()),
                                    m, n, k, out.stride(0), variant, stream))
     return out
+
+
+def gemm_transposed_b_backward(dout: torch.Tensor, A: torch.Tensor, B: torch.Tensor, need_da: bool = True, need_db: bool = True
+                               ) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """Gradients ``(dA, dB)`` of ``gemm_pipeline_transposed_b(A, B)`` from ``dout`` (M, N): ``dA = dout @ B`` (M, K) and
+    ``dB = dout.T @ A`` (N, K), summed in fp32 and rounded to bf16 once.
+
+    The operands are read as they lie in memory (no transposed copies); any 16-byte aligned row stride will do.  N and K must be
+    multiples of 8, M is free.  ``need_da=False`` / ``need_db=False`` leave that product out and return None in its place.
+    """
+    lda = _dense.matrix(A, "A", torch.bfloat16)
+    m, k = A.shape
+    dev = A.device
+    ldb = _dense.matrix(B, "B", torch.bfloat16, None, dev)
+    n = B.shape[0]
+    if B.shape[1] != k:
+        raise ValueError(f"A and B must share K, got {k} and {B.shape[1]}.")
+    _dense.multiple(n, "N", GROUP_N)
+    _dense.multiple(k, "K", GROUP_K, positive=True)
+    ldo = _dense.matrix(dout, "dout", torch.bfloat16, (m, n), dev)
+    da = torch.empty((m, k), dtype=torch.bfloat16, device=dev) if need_da else None
+    db = torch.empty((n, k), dtype=torch.bfloat16, device=dev) if need_db else None
+    if m and n:
+        if need_da or need_db:
+            _dense.call("ave_bf16_gemm_backward", dev, dout.data_ptr(), ldo, A.data_ptr(), lda, B.data_ptr(), ldb,
+                        da.data_ptr() if need_da else None, k, db.data_ptr() if need_db else None, k, m, n, k)
+    else:      # an empty sum
+        for d in (da, db):
+            if d is not None:
+                d.zero_()
+    return da, db

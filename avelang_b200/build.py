@@ -9,17 +9,20 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.path.join(_HERE, "libavefp4.so")
-SOURCES = ["ave_fp4_api.cu"]
-HEADERS = ["sm100_ptx.cuh", "gemm_fp4_sm100.cuh", "gemm_fp4_skinny_sm100.cuh", "quantize_fp4.cuh"]
+SOURCES = ["ave_fp4_api.cu", "ave_dense_api.cu"]
+HEADERS = ["sm100_ptx.cuh", "gemm_fp4_sm100.cuh", "gemm_fp4_skinny_sm100.cuh", "quantize_fp4.cuh", "host_shared.h",
+           "activations.cuh", "gemm_dense_sm100.cuh", "gemm_stream_sm100.cuh", "quantize_int8.cuh", "gated_backward.cuh"]
+ABI_HEADERS = ["ave_fp4.h", "ave_dense.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC",
+    "-Xcompiler", "-fPIC",
 ]
 
 
@@ -35,7 +38,7 @@ def is_stale() -> bool:
         return True
     built = os.path.getmtime(LIB_PATH)
     deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(_HERE, "..", "include", "ave_fp4.h"))
+    deps += [os.path.join(_HERE, "..", "include", f) for f in ABI_HEADERS]
     return any(os.path.getmtime(d) > built for d in deps)
 
 
@@ -43,15 +46,21 @@ def build(force: bool = False, verbose: bool = False) -> str:
     """Compile the library if it is missing or older than its sources; return its path."""
     if not force and not is_stale():
         return LIB_PATH
-    cmd = [_nvcc(), *NVCC_FLAGS]
+    flags = [*NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else [])]
+    with tempfile.TemporaryDirectory() as tmp:
+        # one object per source, compiled side by side, then one link
+        objects = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        jobs = [subprocess.Popen([_nvcc(), *flags, "-c", "-o", o, os.path.join(CSRC, s)], stdout=subprocess.PIPE,
+                                 stderr=subprocess.STDOUT, text=True) for s, o in zip(SOURCES, objects)]
+        outs = [job.communicate()[0] for job in jobs]
+        if any(job.returncode != 0 for job in jobs):
+            raise RuntimeError("nvcc failed:\n" + "".join(outs))
+        link = subprocess.run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB_PATH, *objects], stdout=subprocess.PIPE,
+                              stderr=subprocess.STDOUT, text=True)
+    if link.returncode != 0:
+        raise RuntimeError("nvcc failed:\n" + link.stdout)
     if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", LIB_PATH, *[os.path.join(CSRC, s) for s in SOURCES]]
-    proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + proc.stdout)
-    if verbose:
-        print(proc.stdout)
+        print("".join(outs))
     return LIB_PATH
 
 

@@ -1,0 +1,525 @@
+// Host side of include/ave_dense.h: argument checks, tile choice and launches of the integer, gated and gradient kernels.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdarg>
+#include <cstdio>
+#include <cstring>
+
+#include "../../include/ave_dense.h"
+#include "gated_backward.cuh"
+#include "gemm_dense_sm100.cuh"
+#include "gemm_stream_sm100.cuh"
+#include "host_shared.h"
+#include "quantize_int8.cuh"
+
+namespace {
+
+using namespace avefp4;
+
+int fail(const char* fmt, ...) {
+    char text[256];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(text, sizeof(text), fmt, ap);
+    va_end(ap);
+    return host_fail(-AVE_FP4_ERR_ARG, text);
+}
+
+#define AVE_CUDA(call)                                              \
+    do {                                                            \
+        cudaError_t e__ = (call);                                   \
+        if (e__ != cudaSuccess) return host_fail_cuda(e__, #call);  \
+    } while (0)
+
+constexpr int64_t kMaxDim = int64_t(1) << 28;     // keeps byte coordinates of a tensor map inside 32 bits
+
+bool sizes_ok(int64_t a, int64_t b, int64_t c) {
+    return a >= 0 && b >= 0 && c >= 0 && a <= kMaxDim && b <= kMaxDim && c <= kMaxDim;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// A row-major matrix of `elem`-byte elements: pointer and row stride on 16 bytes, rows not overlapping.
+int check_matrix(const char* fn, const char* name, const void* p, int64_t rows, int64_t cols, int64_t ld, int elem) {
+    if (p == nullptr || !aligned16(p)) return fail("%s: %s is null or not 16-byte aligned", fn, name);
+    if (rows > 1 && (ld < cols || ld % (16 / elem) != 0 || ld > (int64_t(1) << 36)))
+        return fail("%s: the row stride of %s must be at least %lld and a multiple of %d, got %lld", fn, name, static_cast<long long>(cols),
+                    16 / elem, static_cast<long long>(ld));
+    return 0;
+}
+
+int check_vector(const char* fn, const char* name, const void* p) {
+    if (p == nullptr || !aligned16(p)) return fail("%s: %s is null or not 16-byte aligned", fn, name);
+    return 0;
+}
+
+int check_activation(const char* fn, int act) {
+    if (act < AVE_FP4_ACT_NONE || act > AVE_FP4_ACT_SILU) return fail("%s: unknown activation %d", fn, act);
+    return 0;
+}
+
+int64_t row_stride(int64_t rows, int64_t cols, int64_t ld) { return rows > 1 ? ld : cols; }
+
+// Launch attributes: CTA pairs, and the next kernel's launch and set-up under this one's tail (each kernel here waits for the
+// previous grid on the device before it touches global memory).
+struct Launch {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    Launch(int64_t grid, int threads, size_t smem, int cluster, cudaStream_t stream) {
+        memset(&cfg, 0, sizeof(cfg));
+        cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+        cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attr[1].val.clusterDim.y = 1;
+        attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = cluster > 1 ? 2 : 1;
+    }
+};
+
+// ------------------------------------------------------------------------------- tile kernel
+struct Operand {
+    const void* p;
+    int64_t ld;
+};
+
+// Columns of a tile: whole waves first.  A launch takes (waves) x (time of a tile), and the tile's time goes with its
+// columns plus a share that does not (hand-over, the A panel).
+int choose_block_n(int64_t cols, int64_t tile_rows, int64_t clusters, int step) {
+    int best = 256;
+    int64_t best_cost = INT64_MAX;
+    for (int bn = 256; bn >= 64; bn -= step) {
+        const int64_t tiles = tile_rows * ((cols + bn - 1) / bn);
+        const int64_t cost = (tiles + clusters - 1) / clusters * (bn + 32);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = bn;
+        }
+    }
+    return best;
+}
+
+// m, n: result sizes (of one result); k: sum length of one segment.  a[1] / b[1]: second operand of two segments, two
+// results, or the second weight of the gated form.
+template <int CG, int OP, int EPI>
+int launch_dense(const HostDevice& dev, const Operand (&a)[2], const Operand (&b)[2], int64_t m, int64_t n, int64_t k,
+                 DenseParams p, cudaStream_t stream) {
+    using Cfg = DenseConfig<CG>;
+    constexpr bool kAMn = (OP == kOpBf16Tn), kBMn = (OP == kOpBf16Nn || OP == kOpBf16Tn);
+    constexpr int kElem = (OP == kOpInt8) ? 1 : 2;
+    constexpr int kBlockK = 128 / kElem;
+    p.m = static_cast<int>(m);
+    p.n = static_cast<int>(n);
+    p.num_kb = static_cast<int>((k + kBlockK - 1) / kBlockK);
+    p.tiles_m = static_cast<int>((m + 128 * CG - 1) / (128 * CG));
+    const int64_t clusters = dev.sm_count / CG;
+    const int64_t cols = (EPI == kDenseGated) ? 2 * n : n;
+    p.block_n = choose_block_n(cols, int64_t(p.tiles_m) * p.batches, clusters, kBMn ? 64 * CG : (EPI == kDenseGated || CG == 2) ? 32 : 16);
+    const int out_cols = (EPI == kDenseGated) ? p.block_n / 2 : p.block_n;
+    p.tiles_n = static_cast<int>((n + out_cols - 1) / out_cols);
+    p.band = 8;
+    p.status = dev.status;
+    p.pdl = 1;
+
+    CUtensorMap ta[2], tb[2];
+    const int b_rows = (EPI == kDenseGated) ? out_cols : p.block_n / CG;
+    for (int i = 0; i < 2; ++i) {
+        int rc;
+        if (kAMn) rc = host_encode_bytes(&ta[i], a[i].p, m * kElem, k, a[i].ld * kElem, 64, "A");
+        else rc = host_encode_bytes(&ta[i], a[i].p, k * kElem, m, a[i].ld * kElem, 128, "A");
+        if (rc) return rc;
+        if (kBMn) rc = host_encode_bytes(&tb[i], b[i].p, n * kElem, k, b[i].ld * kElem, 64, "B");
+        else rc = host_encode_bytes(&tb[i], b[i].p, k * kElem, n, b[i].ld * kElem, b_rows, "B");
+        if (rc) return rc;
+    }
+    const int64_t tiles = int64_t(p.tiles_m) * p.batches * p.tiles_n;
+    Launch launch((tiles < clusters ? tiles : clusters) * CG, Cfg::kThreads, Cfg::kSmemBytes, CG, stream);
+    AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gemm_dense_kernel<CG, OP, EPI>, ta[0], ta[1], tb[0], tb[1], p));
+    return 0;
+}
+
+template <int OP, int EPI>
+int launch_dense_rows(const HostDevice& dev, const Operand (&a)[2], const Operand (&b)[2], int64_t m, int64_t n, int64_t k,
+                      const DenseParams& p, cudaStream_t stream) {
+    // up to 128 rows fill one CTA's tile: all SMs then take columns of their own instead of half a pair's empty rows
+    if (m <= 128) return launch_dense<1, OP, EPI>(dev, a, b, m, n, k, p, stream);
+    return launch_dense<2, OP, EPI>(dev, a, b, m, n, k, p, stream);
+}
+
+DenseParams dense_params() {
+    DenseParams p;
+    memset(&p, 0, sizeof(p));
+    p.segments = 1;
+    p.batches = 1;
+    return p;
+}
+
+// ------------------------------------------------------------------------------ a few tokens
+constexpr int64_t kStreamMaxM = 16;
+
+template <bool INT8, bool GATED, int ROWS>
+int launch_stream(const StreamParams& p, cudaStream_t stream) {
+    const int out = GATED ? ROWS / 2 : ROWS;
+    Launch launch((p.n + out - 1) / out, kStreamWarps * 32, 0, 1, stream);
+    if (p.m <= 8) AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gemm_stream_kernel<INT8, GATED, true, ROWS>, p));
+    else AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gemm_stream_kernel<INT8, GATED, false, ROWS>, p));
+    return 0;
+}
+
+StreamParams stream_params(const void* x, int64_t ldx_bytes, int64_t m, int64_t n, int64_t k_bytes, int act, void* d, int64_t ldd) {
+    StreamParams p;
+    memset(&p, 0, sizeof(p));
+    p.x = static_cast<const uint8_t*>(x);
+    p.ldx = ldx_bytes;
+    p.m = static_cast<int>(m);
+    p.n = static_cast<int>(n);
+    p.k_bytes = static_cast<int>(k_bytes);
+    p.act = act;
+    p.pdl = 1;
+    p.d = static_cast<__nv_bfloat16*>(d);
+    p.ldd = ldd;
+    return p;
+}
+
+template <int NV, bool CTA_ROW>
+int launch_quantize(const void* x, int64_t rows, int64_t k, int64_t ldx, void* values, int64_t ldv, void* scales, cudaStream_t stream) {
+    const int64_t per_cta = CTA_ROW ? 1 : kInt8Threads / 32;
+    Launch launch((rows + per_cta - 1) / per_cta, kInt8Threads, 0, 1, stream);
+    AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, quantize_int8_kernel<NV, CTA_ROW>, static_cast<const __nv_bfloat16*>(x),
+                                static_cast<long long>(rows), static_cast<int>(k), static_cast<long long>(ldx), static_cast<int8_t*>(values),
+                                static_cast<long long>(ldv), static_cast<float*>(scales), 1));
+    return 0;
+}
+
+template <int ACT>
+int launch_gated_backward(const HostDevice& dev, const void* dd, int64_t ld_dd, const void* gate, int64_t ld_gate, const void* up,
+                          int64_t ld_up, void* d_gate, void* d_up, int64_t m, int64_t f, cudaStream_t stream) {
+    const int64_t pieces = m * (f / 8);
+    const int64_t most = int64_t(dev.sm_count) * 8;
+    int64_t grid = (pieces + 255) / 256;
+    if (grid > most) grid = most;
+    Launch launch(grid, 256, 0, 1, stream);
+    AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gated_backward_kernel<ACT>, static_cast<const __nv_bfloat16*>(dd), static_cast<long long>(ld_dd),
+                                static_cast<const __nv_bfloat16*>(gate), static_cast<long long>(ld_gate), static_cast<const __nv_bfloat16*>(up),
+                                static_cast<long long>(ld_up), static_cast<__nv_bfloat16*>(d_gate), static_cast<__nv_bfloat16*>(d_up),
+                                static_cast<long long>(m), static_cast<int>(f / 8), 1));
+    return 0;
+}
+
+int zero_matrix(void* d, int64_t rows, int64_t cols, int64_t ld, cudaStream_t stream) {
+    if (rows == 0 || cols == 0) return 0;
+    AVE_CUDA(cudaMemset2DAsync(d, static_cast<size_t>(row_stride(rows, cols, ld)) * 2, 0, static_cast<size_t>(cols) * 2, static_cast<size_t>(rows), stream));
+    return 0;
+}
+
+}  // namespace
+
+namespace avefp4 {
+
+cudaError_t prepare_dense_kernels() {
+    cudaError_t e;
+#define PREP(CG, OP, EPI)                                                                                                              \
+    if ((e = cudaFuncSetAttribute(gemm_dense_kernel<CG, OP, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, DenseConfig<CG>::kSmemBytes)) != cudaSuccess) \
+        return e;
+    PREP(1, kOpInt8, kDenseScaled)
+    PREP(2, kOpInt8, kDenseScaled)
+    PREP(1, kOpInt8, kDenseGated)
+    PREP(2, kOpInt8, kDenseGated)
+    PREP(1, kOpBf16, kDenseGated)
+    PREP(2, kOpBf16, kDenseGated)
+    PREP(2, kOpBf16Nn, kDensePlain)
+    PREP(2, kOpBf16Tn, kDensePlain)
+#undef PREP
+    return cudaSuccess;
+}
+
+}  // namespace avefp4
+
+#define CHECK(x)              \
+    do {                      \
+        int rc__ = (x);       \
+        if (rc__) return rc__; \
+    } while (0)
+
+extern "C" {
+
+int ave_int8_quantize(const void* x_bf16, int64_t rows, int64_t k, int64_t ldx, void* values, int64_t ldv, void* scales,
+                      void* stream) {
+    static const char* fn = "ave_int8_quantize";
+    HostDevice dev;
+    if (!sizes_ok(rows, k, 0)) return fail("%s: size out of range", fn);
+    if (k == 0 || k % 16 != 0) return fail("%s: K must be a positive multiple of 16, got %lld", fn, static_cast<long long>(k));
+    if (rows == 0) return 0;
+    CHECK(check_matrix(fn, "x", x_bf16, rows, k, ldx, 2));
+    CHECK(check_matrix(fn, "values", values, rows, k, ldv, 1));
+    CHECK(check_vector(fn, "scales", scales));
+    CHECK(host_device(&dev));
+    ldx = row_stride(rows, k, ldx);
+    ldv = row_stride(rows, k, ldv);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (k <= 256) return launch_quantize<1, false>(x_bf16, rows, k, ldx, values, ldv, scales, s);
+    if (k <= 512) return launch_quantize<2, false>(x_bf16, rows, k, ldx, values, ldv, scales, s);
+    if (k <= 1024) return launch_quantize<4, false>(x_bf16, rows, k, ldx, values, ldv, scales, s);
+    if (k <= 2048) return launch_quantize<1, true>(x_bf16, rows, k, ldx, values, ldv, scales, s);
+    if (k <= 4096) return launch_quantize<2, true>(x_bf16, rows, k, ldx, values, ldv, scales, s);
+    if (k <= 8192) return launch_quantize<4, true>(x_bf16, rows, k, ldx, values, ldv, scales, s);
+    if (k <= 16384) return launch_quantize<8, true>(x_bf16, rows, k, ldx, values, ldv, scales, s);
+    return launch_quantize<0, true>(x_bf16, rows, k, ldx, values, ldv, scales, s);
+}
+
+int ave_int8_gemm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, const void* b_scales,
+                  const void* bias_bf16, int activation, void* d_bf16, int64_t ldd, int64_t m, int64_t n, int64_t k, void* stream) {
+    static const char* fn = "ave_int8_gemm";
+    HostDevice dev;
+    if (!sizes_ok(m, n, k)) return fail("%s: size out of range", fn);
+    if (n % 8 != 0) return fail("%s: N must be a multiple of 8, got %lld", fn, static_cast<long long>(n));
+    if (k == 0 || k % 16 != 0 || k > AVE_INT8_MAX_K)
+        return fail("%s: K must be a positive multiple of 16, at most %d, got %lld", fn, AVE_INT8_MAX_K, static_cast<long long>(k));
+    CHECK(check_activation(fn, activation));
+    if (m == 0 || n == 0) return 0;
+    CHECK(check_matrix(fn, "A", a, m, k, lda, 1));
+    CHECK(check_matrix(fn, "B", b, n, k, ldb, 1));
+    CHECK(check_matrix(fn, "D", d_bf16, m, n, ldd, 2));
+    CHECK(check_vector(fn, "the scales of A", a_scales));
+    CHECK(check_vector(fn, "the scales of B", b_scales));
+    if (bias_bf16 != nullptr) CHECK(check_vector(fn, "the bias", bias_bf16));
+    CHECK(host_device(&dev));
+    lda = row_stride(m, k, lda);
+    ldb = row_stride(n, k, ldb);
+    ldd = row_stride(m, n, ldd);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (m <= kStreamMaxM) {
+        StreamParams p = stream_params(a, lda, m, n, k, activation, d_bf16, ldd);
+        p.w[0] = static_cast<const uint8_t*>(b);
+        p.ldw[0] = ldb;
+        p.x_scale = static_cast<const float*>(a_scales);
+        p.w_scale[0] = static_cast<const float*>(b_scales);
+        p.bias = static_cast<const __nv_bfloat16*>(bias_bf16);
+        return n >= 16 * 4 * dev.sm_count ? launch_stream<true, false, 16>(p, s) : launch_stream<true, false, 8>(p, s);
+    }
+    DenseParams p = dense_params();
+    p.a_scale = static_cast<const float*>(a_scales);
+    p.b_scale[0] = p.b_scale[1] = static_cast<const float*>(b_scales);
+    p.bias = static_cast<const __nv_bfloat16*>(bias_bf16);
+    p.act = activation;
+    p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(d_bf16);
+    p.ldd = ldd;
+    return launch_dense_rows<kOpInt8, kDenseScaled>(dev, {{a, lda}, {a, lda}}, {{b, ldb}, {b, ldb}}, m, n, k, p, s);
+}
+
+int ave_int8_gemm_gated(const void* a, int64_t lda, const void* a_scales, const void* w_gate, int64_t ld_wg, const void* gate_scales,
+                        const void* w_up, int64_t ld_wu, const void* up_scales, int activation, void* d_bf16, int64_t ldd,
+                        int64_t m, int64_t f, int64_t k, void* stream) {
+    static const char* fn = "ave_int8_gemm_gated";
+    HostDevice dev;
+    if (!sizes_ok(m, f, k)) return fail("%s: size out of range", fn);
+    if (f % 8 != 0) return fail("%s: F must be a multiple of 8, got %lld", fn, static_cast<long long>(f));
+    if (k == 0 || k % 16 != 0 || k > AVE_INT8_MAX_K)
+        return fail("%s: K must be a positive multiple of 16, at most %d, got %lld", fn, AVE_INT8_MAX_K, static_cast<long long>(k));
+    CHECK(check_activation(fn, activation));
+    if (m == 0 || f == 0) return 0;
+    CHECK(check_matrix(fn, "A", a, m, k, lda, 1));
+    CHECK(check_matrix(fn, "W_gate", w_gate, f, k, ld_wg, 1));
+    CHECK(check_matrix(fn, "W_up", w_up, f, k, ld_wu, 1));
+    CHECK(check_matrix(fn, "D", d_bf16, m, f, ldd, 2));
+    CHECK(check_vector(fn, "the scales of A", a_scales));
+    CHECK(check_vector(fn, "the scales of W_gate", gate_scales));
+    CHECK(check_vector(fn, "the scales of W_up", up_scales));
+    CHECK(host_device(&dev));
+    lda = row_stride(m, k, lda);
+    ld_wg = row_stride(f, k, ld_wg);
+    ld_wu = row_stride(f, k, ld_wu);
+    ldd = row_stride(m, f, ldd);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (m <= kStreamMaxM) {
+        StreamParams p = stream_params(a, lda, m, f, k, activation, d_bf16, ldd);
+        p.w[0] = static_cast<const uint8_t*>(w_gate);
+        p.w[1] = static_cast<const uint8_t*>(w_up);
+        p.ldw[0] = ld_wg;
+        p.ldw[1] = ld_wu;
+        p.x_scale = static_cast<const float*>(a_scales);
+        p.w_scale[0] = static_cast<const float*>(gate_scales);
+        p.w_scale[1] = static_cast<const float*>(up_scales);
+        return launch_stream<true, true, 16>(p, s);
+    }
+    DenseParams p = dense_params();
+    p.a_scale = static_cast<const float*>(a_scales);
+    p.b_scale[0] = static_cast<const float*>(gate_scales);
+    p.b_scale[1] = static_cast<const float*>(up_scales);
+    p.act = activation;
+    p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(d_bf16);
+    p.ldd = ldd;
+    return launch_dense_rows<kOpInt8, kDenseGated>(dev, {{a, lda}, {a, lda}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, k, p, s);
+}
+
+int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t ld_wg, const void* w_up, int64_t ld_wu, int activation,
+                        void* d_bf16, int64_t ldd, void* gate_bf16, int64_t ld_gate, void* up_bf16, int64_t ld_up,
+                        int64_t m, int64_t f, int64_t h, void* stream) {
+    static const char* fn = "ave_bf16_gemm_gated";
+    HostDevice dev;
+    if (!sizes_ok(m, f, h)) return fail("%s: size out of range", fn);
+    if (f % 8 != 0) return fail("%s: F must be a multiple of 8, got %lld", fn, static_cast<long long>(f));
+    if (h == 0 || h % 8 != 0) return fail("%s: H must be a positive multiple of 8, got %lld", fn, static_cast<long long>(h));
+    CHECK(check_activation(fn, activation));
+    if ((gate_bf16 == nullptr) != (up_bf16 == nullptr)) return fail("%s: gate and up are kept together or not at all", fn);
+    if (m == 0 || f == 0) return 0;
+    CHECK(check_matrix(fn, "x", x, m, h, ldx, 2));
+    CHECK(check_matrix(fn, "W_gate", w_gate, f, h, ld_wg, 2));
+    CHECK(check_matrix(fn, "W_up", w_up, f, h, ld_wu, 2));
+    CHECK(check_matrix(fn, "D", d_bf16, m, f, ldd, 2));
+    if (gate_bf16 != nullptr) {
+        CHECK(check_matrix(fn, "gate", gate_bf16, m, f, ld_gate, 2));
+        CHECK(check_matrix(fn, "up", up_bf16, m, f, ld_up, 2));
+    }
+    CHECK(host_device(&dev));
+    ldx = row_stride(m, h, ldx);
+    ld_wg = row_stride(f, h, ld_wg);
+    ld_wu = row_stride(f, h, ld_wu);
+    ldd = row_stride(m, f, ldd);
+    ld_gate = row_stride(m, f, ld_gate);
+    ld_up = row_stride(m, f, ld_up);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (m <= kStreamMaxM) {
+        StreamParams p = stream_params(x, ldx * 2, m, f, h * 2, activation, d_bf16, ldd);
+        p.w[0] = static_cast<const uint8_t*>(w_gate);
+        p.w[1] = static_cast<const uint8_t*>(w_up);
+        p.ldw[0] = ld_wg * 2;
+        p.ldw[1] = ld_wu * 2;
+        p.gate = static_cast<__nv_bfloat16*>(gate_bf16);
+        p.up = static_cast<__nv_bfloat16*>(up_bf16);
+        p.ld_gate = ld_gate;
+        p.ld_up = ld_up;
+        return launch_stream<false, true, 16>(p, s);
+    }
+    DenseParams p = dense_params();
+    p.act = activation;
+    p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(d_bf16);
+    p.ldd = ldd;
+    p.gate = static_cast<__nv_bfloat16*>(gate_bf16);
+    p.up = static_cast<__nv_bfloat16*>(up_bf16);
+    p.ld_gate = ld_gate;
+    p.ld_up = ld_up;
+    return launch_dense_rows<kOpBf16, kDenseGated>(dev, {{x, ldx}, {x, ldx}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, h, p, s);
+}
+
+static int64_t gated_backward_half(int64_t m, int64_t f) { return (m * f * 2 + 255) / 256 * 256; }
+
+int64_t ave_bf16_gated_backward_workspace_bytes(int64_t m, int64_t f) {
+    if (!sizes_ok(m, f, 0)) return fail("ave_bf16_gated_backward_workspace_bytes: size out of range");
+    return 2 * gated_backward_half(m, f);
+}
+
+int ave_bf16_gated_backward(const void* dd, int64_t ld_dd, const void* x, int64_t ldx, const void* w_gate, int64_t ld_wg,
+                            const void* w_up, int64_t ld_wu, const void* gate, int64_t ld_gate, const void* up, int64_t ld_up,
+                            int activation, void* dx, int64_t ld_dx, void* dw_gate, void* dw_up, int64_t ld_dw, void* workspace,
+                            int64_t workspace_bytes, int64_t m, int64_t f, int64_t h, void* stream) {
+    static const char* fn = "ave_bf16_gated_backward";
+    HostDevice dev;
+    if (!sizes_ok(m, f, h)) return fail("%s: size out of range", fn);
+    if (f % 8 != 0) return fail("%s: F must be a multiple of 8, got %lld", fn, static_cast<long long>(f));
+    if (h == 0 || h % 8 != 0) return fail("%s: H must be a positive multiple of 8, got %lld", fn, static_cast<long long>(h));
+    CHECK(check_activation(fn, activation));
+    if ((dw_gate == nullptr) != (dw_up == nullptr)) return fail("%s: dW_gate and dW_up are computed together or not at all", fn);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool want_x = dx != nullptr, want_w = dw_gate != nullptr;
+    if (want_x && m > 0) CHECK(check_matrix(fn, "dx", dx, m, h, ld_dx, 2));
+    if (want_w && f > 0) {
+        CHECK(check_matrix(fn, "dW_gate", dw_gate, f, h, ld_dw, 2));
+        CHECK(check_matrix(fn, "dW_up", dw_up, f, h, ld_dw, 2));
+    }
+    if (m == 0 || f == 0) {
+        if (want_x) CHECK(zero_matrix(dx, m, h, ld_dx, s));
+        if (want_w) {
+            CHECK(zero_matrix(dw_gate, f, h, ld_dw, s));
+            CHECK(zero_matrix(dw_up, f, h, ld_dw, s));
+        }
+        return 0;
+    }
+    CHECK(check_matrix(fn, "dD", dd, m, f, ld_dd, 2));
+    CHECK(check_matrix(fn, "x", x, m, h, ldx, 2));
+    CHECK(check_matrix(fn, "W_gate", w_gate, f, h, ld_wg, 2));
+    CHECK(check_matrix(fn, "W_up", w_up, f, h, ld_wu, 2));
+    CHECK(check_matrix(fn, "gate", gate, m, f, ld_gate, 2));
+    CHECK(check_matrix(fn, "up", up, m, f, ld_up, 2));
+    if (!want_x && !want_w) return 0;
+    const int64_t half = gated_backward_half(m, f);
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || workspace_bytes < 2 * half)
+        return fail("%s: the workspace must be 256-byte aligned and hold %lld bytes", fn, static_cast<long long>(2 * half));
+    CHECK(host_device(&dev));
+    ld_dd = row_stride(m, f, ld_dd);
+    ldx = row_stride(m, h, ldx);
+    ld_wg = row_stride(f, h, ld_wg);
+    ld_wu = row_stride(f, h, ld_wu);
+    ld_gate = row_stride(m, f, ld_gate);
+    ld_up = row_stride(m, f, ld_up);
+    void* d_gate = workspace;
+    void* d_up = static_cast<uint8_t*>(workspace) + half;
+    switch (activation) {
+        case AVE_FP4_ACT_RELU: CHECK(launch_gated_backward<AVE_FP4_ACT_RELU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
+        case AVE_FP4_ACT_GELU: CHECK(launch_gated_backward<AVE_FP4_ACT_GELU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
+        case AVE_FP4_ACT_GELU_TANH: CHECK(launch_gated_backward<AVE_FP4_ACT_GELU_TANH>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
+        case AVE_FP4_ACT_SILU: CHECK(launch_gated_backward<AVE_FP4_ACT_SILU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
+        default: CHECK(launch_gated_backward<AVE_FP4_ACT_NONE>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
+    }
+    if (want_x) {
+        DenseParams p = dense_params();
+        p.segments = 2;
+        p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(dx);
+        p.ldd = row_stride(m, h, ld_dx);
+        CHECK((launch_dense<2, kOpBf16Nn, kDensePlain>(dev, {{d_gate, f}, {d_up, f}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, h, f, p, s)));
+    }
+    if (want_w) {
+        DenseParams p = dense_params();
+        p.batches = 2;
+        p.d[0] = static_cast<__nv_bfloat16*>(dw_gate);
+        p.d[1] = static_cast<__nv_bfloat16*>(dw_up);
+        p.ldd = row_stride(f, h, ld_dw);
+        CHECK((launch_dense<2, kOpBf16Tn, kDensePlain>(dev, {{d_gate, f}, {d_up, f}}, {{x, ldx}, {x, ldx}}, f, h, m, p, s)));
+    }
+    return 0;
+}
+
+int ave_bf16_gemm_backward(const void* dd, int64_t ld_dd, const void* a, int64_t lda, const void* b, int64_t ldb, void* da,
+                           int64_t ld_da, void* db, int64_t ld_db, int64_t m, int64_t n, int64_t k, void* stream) {
+    static const char* fn = "ave_bf16_gemm_backward";
+    HostDevice dev;
+    if (!sizes_ok(m, n, k)) return fail("%s: size out of range", fn);
+    if (n % 8 != 0) return fail("%s: N must be a multiple of 8, got %lld", fn, static_cast<long long>(n));
+    if (k == 0 || k % 8 != 0) return fail("%s: K must be a positive multiple of 8, got %lld", fn, static_cast<long long>(k));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (da != nullptr && m > 0) CHECK(check_matrix(fn, "dA", da, m, k, ld_da, 2));
+    if (db != nullptr && n > 0) CHECK(check_matrix(fn, "dB", db, n, k, ld_db, 2));
+    if (m == 0 || n == 0) {
+        if (da != nullptr) CHECK(zero_matrix(da, m, k, ld_da, s));
+        if (db != nullptr) CHECK(zero_matrix(db, n, k, ld_db, s));
+        return 0;
+    }
+    CHECK(check_matrix(fn, "dD", dd, m, n, ld_dd, 2));
+    CHECK(check_matrix(fn, "A", a, m, k, lda, 2));
+    CHECK(check_matrix(fn, "B", b, n, k, ldb, 2));
+    CHECK(host_device(&dev));
+    ld_dd = row_stride(m, n, ld_dd);
+    lda = row_stride(m, k, lda);
+    ldb = row_stride(n, k, ldb);
+    if (da != nullptr) {
+        DenseParams p = dense_params();
+        p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(da);
+        p.ldd = row_stride(m, k, ld_da);
+        CHECK((launch_dense<2, kOpBf16Nn, kDensePlain>(dev, {{dd, ld_dd}, {dd, ld_dd}}, {{b, ldb}, {b, ldb}}, m, k, n, p, s)));
+    }
+    if (db != nullptr) {
+        DenseParams p = dense_params();
+        p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(db);
+        p.ldd = row_stride(n, k, ld_db);
+        CHECK((launch_dense<2, kOpBf16Tn, kDensePlain>(dev, {{dd, ld_dd}, {dd, ld_dd}}, {{a, lda}, {a, lda}}, n, k, m, p, s)));
+    }
+    return 0;
+}
+
+}  // extern "C"

@@ -17,6 +17,7 @@
 #include "../../include/ave_fp4.h"
 #include "gemm_fp4_skinny_sm100.cuh"
 #include "gemm_fp4_sm100.cuh"
+#include "host_shared.h"
 #include "quantize_fp4.cuh"
 
 namespace {
@@ -648,6 +649,27 @@ extern "C" int ave_fp4_gemm_decode_noalloc(const void* a_packed, const void* a_s
 }
 
 // ====================================================================================
+namespace avefp4 {
+
+int host_fail(int code, const char* message) { return fail(code, "%s", message); }
+
+int host_fail_cuda(cudaError_t e, const char* what) { return fail_cuda(e, what); }
+
+int host_device(HostDevice* out) {
+    DeviceState* ds = nullptr;
+    const int rc = current_state(&ds);
+    if (rc) return rc;
+    out->sm_count = ds->sm_count;
+    out->status = ds->status;
+    return 0;
+}
+
+int host_encode_bytes(CUtensorMap* tm, const void* base, uint64_t inner, uint64_t outer, uint64_t stride, uint32_t box_rows, const char* what) {
+    return encode_2d(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, inner, outer, stride, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B, what);
+}
+
+}  // namespace avefp4
+
 extern "C" {
 
 const char* ave_fp4_last_error(void) { return g_err; }
@@ -683,6 +705,7 @@ int ave_fp4_init(int device) {
         g_encode = reinterpret_cast<EncodeTiledFn>(fn);
     }
     AVE_CUDA(prepare_all());
+    AVE_CUDA(prepare_dense_kernels());
     AVE_CUDA(cudaMalloc(&restore.status, sizeof(int)));
     AVE_CUDA(cudaMemset(restore.status, 0, sizeof(int)));
     g_dev[device].status = restore.status;

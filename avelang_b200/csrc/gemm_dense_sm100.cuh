@@ -1,0 +1,419 @@
+// Persistent tcgen05 tile kernel of the dense products that come with something around them:
+//
+//   kOpInt8    C = A B^T       A (M,K), B (N,K) int8, both K-contiguous; int32 accumulators (tcgen05.mma kind::i8)
+//   kOpBf16    C = A B^T       the same for bf16 (kind::f16, fp32 accumulators)
+//   kOpBf16Nn  C = A B         A (M,K), B (K,N) bf16 as they lie in memory: B is read as an MN-major operand
+//   kOpBf16Tn  C = A^T B       A (K,M), B (K,N) bf16: both operands MN-major
+//
+// and, per kernel, one epilogue:
+//
+//   kDensePlain   D = bf16(C)
+//   kDenseScaled  D = bf16(act(C * a_scale[row] * b_scale[col] + bias[col]))
+//   kDenseGated   two weights of F rows each: D = bf16(act(G) * U), G = A Wg^T, U = A Wu^T (with scales for int8);
+//                 optionally G and U are written as bf16 as well, for the backward pass
+//
+// The gated form costs no more than a plain product with 2F columns: half of an accumulator tile's columns are rows of
+// Wg and the other half the rows of Wu with the same numbers, so that the epilogue finds both factors of an output
+// in one thread's TMEM lane.  With CTA pairs this takes no extra load: each CTA supplies half of the B tile, one of
+// them from Wg, the other from Wu.
+//
+// Structure: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue; a ring of shared-memory stages of 128 bytes of
+// K per row (128-byte swizzle); two accumulators of up to 256 columns in TMEM, so a tile's epilogue runs under the next
+// tile's main loop.  The tile is 128 rows per CTA by `block_n` columns, and block_n is a run-time value: the number of
+// columns goes into the instruction descriptor, so the host picks it for whole waves (see choose_block_n).
+//
+// An MN-major operand tile is kept as boxes of 64 elements (one swizzled 128-byte row) x 64 K rows, 8 KB each: the
+// matrix descriptor steps 8 KB from one box to the next along MN (leading offset) and 1 KB from one group of eight
+// K rows to the next (stride offset); an MMA's 16 K rows are two such groups.
+#pragma once
+
+#include "activations.cuh"
+#include "sm100_ptx.cuh"
+
+namespace avefp4 {
+
+enum DenseOperands : int { kOpBf16 = 0, kOpInt8 = 1, kOpBf16Nn = 2, kOpBf16Tn = 3 };
+enum DenseEpilogue : int { kDensePlain = 0, kDenseScaled = 1, kDenseGated = 2 };
+
+struct DenseParams {
+    long long ldd, ld_gate, ld_up;   // row strides in elements
+    int m, n;                        // rows and columns of one result (gated: n = F)
+    int num_kb;                      // K blocks of one segment (64 bf16 or 128 int8 elements of K each)
+    int segments;                    // 2: C = A0 B0 + A1 B1, two operand pairs of the same sizes
+    int batches;                     // 2: two results, C0 from A0 and C1 from A1, B shared; tile rows of C1 follow those of C0
+    int tiles_m, tiles_n;            // tiles of one result
+    int block_n;                     // accumulator columns of a tile
+    int band;                        // tile rows per band of the schedule
+    __nv_bfloat16* d[2];
+    const float* a_scale;            // one per row of A
+    const float* b_scale[2];         // one per row of B; gated: of Wg and Wu
+    const __nv_bfloat16* bias;
+    int act;
+    int pdl;                         // launched with programmatic stream serialisation
+    __nv_bfloat16* gate;             // gated: where to keep G and U, or nullptr
+    __nv_bfloat16* up;
+    int* status;
+};
+
+template <int CG>
+struct DenseConfig {
+    static constexpr int kMaxN = 256;
+    static constexpr int kABytes = 128 * 128;
+    static constexpr int kBBytes = kMaxN / CG * 128;
+    static constexpr int kStages = (CG == 2) ? 6 : 4;
+    static constexpr int kEpiWarps = 8;
+    static constexpr int kEpiBufBytes = 32 * 128;
+    static constexpr int kOffA = 0;
+    static constexpr int kOffB = kStages * kABytes;
+    static constexpr int kOffEpi = kOffB + kStages * kBBytes;
+    static constexpr int kOffBar = kOffEpi + kEpiWarps * kEpiBufBytes;
+    static constexpr int kOffTmemPtr = kOffBar + (2 * kStages + 4) * 8;
+    static constexpr int kSmemBytes = kOffTmemPtr + 16 + 1024;
+    static constexpr int kThreads = 64 + 32 * kEpiWarps;
+    static_assert(kSmemBytes <= 232448, "shared memory budget");
+};
+
+// Instruction descriptor of kind::f16 / kind::i8: bits 4-5 accumulator (1 fp32, 2 int32), 7-9 / 10-12 operand formats
+// (kind::f16: 1 = bf16; kind::i8: 1 = signed), 15 / 16 A / B MN-major, 17-22 N >> 3, 24-28 M >> 4.
+__device__ __forceinline__ uint32_t make_idesc_dense(bool int8, bool a_mn, bool b_mn, int mma_m, int mma_n) {
+    return ((int8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn) << 15) |
+           (static_cast<uint32_t>(b_mn) << 16) | (static_cast<uint32_t>(mma_n >> 3) << 17) |
+           (static_cast<uint32_t>(mma_m >> 4) << 24);
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_int8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 1) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+    }
+}
+
+// Tile number -> (tile row, tile column): bands of `band` tile rows, rows fastest inside a band, so that the CTAs
+// running at the same time share a few A panels and a few B panels in L2.
+__device__ __forceinline__ void dense_tile(int t, int rows, int cols, int band, int& tm, int& tn) {
+    const int per_band = band * cols;
+    const int g = t / per_band;
+    const int first = g * band;
+    const int in_band = min(rows - first, band);
+    const int r = t - g * per_band;
+    tm = first + r % in_band;
+    tn = r / in_band;
+}
+
+// 32 accumulator columns of this thread's row -> 16 words of bf16 pairs.  `col` is the first one's column in the result.
+template <bool INT8, int EPI, int ACT>
+__device__ __forceinline__ void dense_convert(const uint32_t (&v)[32], const uint32_t (&u)[32], uint32_t (&w)[16], float sa,
+                                              const float* sb0, const float* sb1, const __nv_bfloat16* bias, int col, int n) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        float4 s0 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), s1 = s0;
+        float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (col + 4 * q < n) {          // n is a multiple of 8
+            if constexpr (INT8) {
+                s0 = __ldg(reinterpret_cast<const float4*>(sb0 + col) + q);
+                if constexpr (EPI == kDenseGated) s1 = __ldg(reinterpret_cast<const float4*>(sb1 + col) + q);
+            }
+            if constexpr (EPI == kDenseScaled) {
+                if (bias != nullptr) {
+                    const uint2 bw = __ldg(reinterpret_cast<const uint2*>(bias + col) + q);
+                    b[0] = bf16_lo(bw.x); b[1] = bf16_hi(bw.x); b[2] = bf16_lo(bw.y); b[3] = bf16_hi(bw.y);
+                }
+            }
+        }
+        const float c0[4] = {s0.x, s0.y, s0.z, s0.w}, c1[4] = {s1.x, s1.y, s1.z, s1.w};
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            // int32 -> fp32 rounds to nearest: 2^-24 of the sum, far below the one rounding to bf16.  The channel's scale comes
+            // first: weights are of ordinary size, so the product with a large token's scale overflows only if the result does.
+            float g = INT8 ? __int2float_rn(static_cast<int>(v[4 * q + i])) * c0[i] * sa : __uint_as_float(v[4 * q + i]);
+            if constexpr (EPI == kDenseScaled) g += b[i];
+            y[i] = act_value<ACT>(g);
+            if constexpr (EPI == kDenseGated)
+                y[i] *= INT8 ? __int2float_rn(static_cast<int>(u[4 * q + i])) * c1[i] * sa : __uint_as_float(u[4 * q + i]);
+        }
+        w[2 * q] = pack_bf16(y[0], y[1]);
+        w[2 * q + 1] = pack_bf16(y[2], y[3]);
+    }
+}
+
+template <int CG, int OP, int EPI>
+__global__ void __launch_bounds__(320, 1)
+gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constant__ CUtensorMap tm_a1,
+                  const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1, const DenseParams p) {
+    using Cfg = DenseConfig<CG>;
+    constexpr int STAGES = Cfg::kStages;
+    constexpr bool kInt8 = (OP == kOpInt8);
+    constexpr bool kAMn = (OP == kOpBf16Tn);
+    constexpr bool kBMn = (OP == kOpBf16Nn || OP == kOpBf16Tn);
+    constexpr bool kGated = (EPI == kDenseGated);
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+
+    // warp-uniform values through a shuffle, so that the issue loops keep them in uniform registers
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+    const int lane = threadIdx.x & 31;
+    const int rank = (CG == 2) ? static_cast<int>(__shfl_sync(0xffffffffu, cluster_ctarank(), 0)) : 0;
+    const bool is_leader = (rank == 0);
+    const int cluster_id = blockIdx.x / CG;
+    const int num_clusters = gridDim.x / CG;
+    const int tile_rows = p.tiles_m * p.batches;
+    const int num_tiles = tile_rows * p.tiles_n;
+    const int num_kb = p.num_kb * p.segments;
+    const int bn_cta = p.block_n / CG;                            // rows of B that one CTA loads
+    const int out_cols = kGated ? p.block_n / 2 : p.block_n;      // result columns of a tile
+
+    const uint32_t bar_full = smem_base + Cfg::kOffBar;
+    const uint32_t bar_empty = bar_full + STAGES * 8;
+    const uint32_t bar_tfull = bar_empty + STAGES * 8;
+    const uint32_t bar_tempty = bar_tfull + 2 * 8;
+    const uint32_t tmem_ptr_smem = smem_base + Cfg::kOffTmemPtr;
+    volatile uint32_t* tmem_ptr_gen = reinterpret_cast<volatile uint32_t*>(smem_gen + Cfg::kOffTmemPtr);
+
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&tm_a0);
+        prefetch_tensormap(&tm_b0);
+        prefetch_tensormap(&tm_a1);
+        prefetch_tensormap(&tm_b1);
+        for (int s = 0; s < STAGES; ++s) {
+            mbar_init(bar_full + s * 8, 1);
+            mbar_init(bar_empty + s * 8, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(bar_tfull + a * 8, 1);
+            mbar_init(bar_tempty + a * 8, Cfg::kEpiWarps * CG);
+        }
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        tmem_alloc<CG>(tmem_ptr_smem, 512);
+        tmem_relinquish<CG>();
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync_all();
+    tcgen05_fence_after();
+    const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_gen, 0);
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        const bool issuer = elect_one_sync();
+        if (p.pdl) {
+            if (issuer) pdl_launch_dependents();
+            pdl_wait_prior_grid();       // operands may come from the previous kernel
+        }
+        const uint32_t full0 = (CG == 2) ? mapa_shared(bar_full, 0) : bar_full;
+        const uint32_t tx_bytes = static_cast<uint32_t>(CG * (Cfg::kABytes + bn_cta * 128));
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = cluster_id; t < num_tiles && ok; t += num_clusters) {
+            int tm, tn;
+            dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn);
+            const bool second = tm >= p.tiles_m;                  // tile of the second result
+            const int row_a = ((second ? tm - p.tiles_m : tm) * CG + rank) * 128;
+            const int row_b = tn * out_cols + (kGated ? 0 : rank * bn_cta);
+            int seg = 0, kb = 0;
+            for (int i = 0; i < num_kb; ++i) {
+                if (!mbar_wait(bar_empty + stage * 8, phase ^ 1u)) {
+                    if (issuer) atomicCAS(p.status, 0, 101);
+                    ok = false;
+                    break;
+                }
+                if (issuer) {
+                    const uint32_t full = full0 + stage * 8;
+                    const uint32_t sa = smem_base + Cfg::kOffA + stage * Cfg::kABytes;
+                    const uint32_t sb = smem_base + Cfg::kOffB + stage * Cfg::kBBytes;
+                    const CUtensorMap* ta = (second || seg) ? &tm_a1 : &tm_a0;
+                    const CUtensorMap* tb = seg ? &tm_b1 : &tm_b0;
+                    if (is_leader) mbar_arrive_expect_tx(bar_full + stage * 8, tx_bytes);
+                    if constexpr (kAMn) {
+                        tma_load_2d<CG, 2>(sa, ta, full, row_a * 2, kb * 64);
+                        tma_load_2d<CG, 2>(sa + 8192, ta, full, row_a * 2 + 128, kb * 64);
+                    } else {
+                        tma_load_2d<CG, 2>(sa, ta, full, kb * 128, row_a);
+                    }
+                    if constexpr (kBMn) {
+                        for (int c = 0; c < bn_cta; c += 64)
+                            tma_load_2d<CG, 2>(sb + c * 128, tb, full, (row_b + c) * 2, kb * 64);
+                    } else if constexpr (kGated && CG == 2) {
+                        tma_load_2d<CG, 2>(sb, rank ? &tm_b1 : &tm_b0, full, kb * 128, row_b);
+                    } else if constexpr (kGated) {
+                        tma_load_2d<CG, 2>(sb, &tm_b0, full, kb * 128, row_b);
+                        tma_load_2d<CG, 2>(sb + out_cols * 128, &tm_b1, full, kb * 128, row_b);
+                    } else {
+                        tma_load_2d<CG, 2>(sb, tb, full, kb * 128, row_b);
+                    }
+                }
+                if (++kb == p.num_kb) { kb = 0; ++seg; }
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+        }
+        if (ok) {
+            // wait until every filled stage has been consumed: no copy or signal is outstanding when the CTA exits
+            for (int i = 0; i < STAGES; ++i) {
+                if (!mbar_wait(bar_empty + stage * 8, phase ^ 1u)) {
+                    if (issuer) atomicCAS(p.status, 0, 101);
+                    break;
+                }
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------- MMA issuer
+        if (is_leader) {
+            const bool issuer = elect_one_sync();
+            const uint32_t idesc = make_idesc_dense(kInt8, kAMn, kBMn, 128 * CG, p.block_n);
+            int stage = 0;
+            uint32_t phase = 0;
+            int tile_iter = 0;
+            bool ok = true;
+            for (int t = cluster_id; t < num_tiles && ok; t += num_clusters, ++tile_iter) {
+                const int acc = tile_iter & 1;
+                const uint32_t acc_phase = static_cast<uint32_t>(tile_iter >> 1) & 1u;
+                if (!mbar_wait(bar_tempty + acc * 8, acc_phase ^ 1u)) {
+                    if (issuer) atomicCAS(p.status, 0, 102);
+                    ok = false;
+                    break;
+                }
+                tcgen05_fence_after();
+                const uint32_t d_tmem = tmem_base + acc * 256;
+                for (int i = 0; i < num_kb; ++i) {
+                    if (!mbar_wait(bar_full + stage * 8, phase)) {
+                        if (issuer) atomicCAS(p.status, 0, 102);
+                        ok = false;
+                        break;
+                    }
+                    tcgen05_fence_after();
+                    const uint32_t sa = smem_base + Cfg::kOffA + stage * Cfg::kABytes;
+                    const uint32_t sb = smem_base + Cfg::kOffB + stage * Cfg::kBBytes;
+                    const uint64_t a_desc = kAMn ? make_smem_desc(sa, 8192, 1024, 2) : make_desc_k_sw128(sa);
+                    const uint64_t b_desc = kBMn ? make_smem_desc(sb, 8192, 1024, 2) : make_desc_k_sw128(sb);
+                    if (issuer) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            // descriptor addresses count 16 bytes: a K step is 32 bytes along a K-major row, or 16 K rows
+                            // (2 KB) of an MN-major tile
+                            const uint64_t ad = a_desc + static_cast<uint64_t>(j * (kAMn ? 128 : 2));
+                            const uint64_t bd = b_desc + static_cast<uint64_t>(j * (kBMn ? 128 : 2));
+                            const uint32_t accumulate = (i > 0 || j > 0) ? 1u : 0u;
+                            if constexpr (kInt8) mma_int8<CG>(d_tmem, ad, bd, idesc, accumulate);
+                            else mma_bf16<CG>(d_tmem, ad, bd, idesc, accumulate);
+                        }
+                        tcgen05_commit<CG>(bar_empty + stage * 8);
+                    }
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+                if (ok && issuer) tcgen05_commit<CG>(bar_tfull + acc * 8);
+                __syncwarp();
+            }
+        }
+    } else {
+        // --------------------------------------------------------------- epilogue
+        const int quad = warp & 3;             // TMEM lane quadrant this warp may access
+        const int half = (warp - 2) >> 2;      // takes every second group of 64 result columns
+        const uint32_t sbuf = smem_base + Cfg::kOffEpi + (warp - 2) * Cfg::kEpiBufBytes;
+        if (p.pdl) pdl_wait_prior_grid();
+        const uint32_t tempty0 = (CG == 2) ? mapa_shared(bar_tempty, 0) : bar_tempty;
+        const int results = (kGated && p.gate != nullptr) ? 3 : 1;
+        int tile_iter = 0;
+        for (int t = cluster_id; t < num_tiles; t += num_clusters, ++tile_iter) {
+            int tm, tn;
+            dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn);
+            const bool second = tm >= p.tiles_m;
+            const int acc = tile_iter & 1;
+            const uint32_t acc_phase = static_cast<uint32_t>(tile_iter >> 1) & 1u;
+            const int row0 = ((second ? tm - p.tiles_m : tm) * CG + rank) * 128 + quad * 32;
+            const int col0 = tn * out_cols;
+            float sa = 1.0f;
+            if constexpr (kInt8) sa = (row0 + lane < p.m) ? __ldg(p.a_scale + row0 + lane) : 0.0f;
+            if (!mbar_wait(bar_tfull + acc * 8, acc_phase)) {
+                if (lane == 0) atomicCAS(p.status, 0, 103);
+                break;
+            }
+            tcgen05_fence_after();
+            const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * 256;
+            for (int c0 = half * 64; c0 < out_cols; c0 += 128) {
+                for (int r = 0; r < results; ++r) {
+                    // 32 rows x 64 columns through a swizzled transpose: lane = row, 16-byte chunk q of a row lives at
+                    // chunk q ^ (row & 7); every store below then writes whole 128-byte lines
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        const int c = c0 + h * 32;
+                        if (c >= out_cols) break;
+                        uint32_t v[32], u[32], w[16];
+                        if (!kGated || r < 2) tmem_ld_32x32b_x32(t_acc + c, v);
+                        if constexpr (kGated) {
+                            if (r == 0) tmem_ld_32x32b_x32(t_acc + out_cols + c, u);
+                            if (r == 2) tmem_ld_32x32b_x32(t_acc + out_cols + c, v);
+                        }
+                        tmem_ld_wait();
+                        if (kGated && r > 0) {
+                            dense_convert<false, kDensePlain, AVE_FP4_ACT_NONE>(v, v, w, sa, nullptr, nullptr, nullptr, col0 + c, p.n);
+                        } else if constexpr (EPI == kDensePlain) {
+                            dense_convert<false, kDensePlain, AVE_FP4_ACT_NONE>(v, v, w, sa, nullptr, nullptr, nullptr, col0 + c, p.n);
+                        } else {
+                            switch (p.act) {   // warp-uniform
+                                case AVE_FP4_ACT_RELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_RELU>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
+                                case AVE_FP4_ACT_GELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
+                                case AVE_FP4_ACT_GELU_TANH: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU_TANH>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
+                                case AVE_FP4_ACT_SILU: dense_convert<kInt8, EPI, AVE_FP4_ACT_SILU>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
+                                default: dense_convert<kInt8, EPI, AVE_FP4_ACT_NONE>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
+                            }
+                        }
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const uint32_t addr = sbuf + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4);
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[4 * q]), "r"(w[4 * q + 1]),
+                                         "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
+                                         : "memory");
+                        }
+                    }
+                    __syncwarp();
+                    __nv_bfloat16* d = p.d[second ? 1 : 0];
+                    long long ld = p.ldd;
+                    if (kGated && r == 1) { d = p.gate; ld = p.ld_gate; }
+                    if (kGated && r == 2) { d = p.up; ld = p.ld_up; }
+                    const int q = lane & 7;
+                    const int c = c0 + q * 8;
+                    const bool col_ok = (c < out_cols) && (col0 + c < p.n);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int rr = i * 4 + (lane >> 3);
+                        const uint32_t addr = sbuf + rr * 128 + ((q ^ (rr & 7)) << 4);
+                        uint32_t w0, w1, w2, w3;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3) : "r"(addr) : "memory");
+                        if (col_ok && row0 + rr < p.m)
+                            __stcs(reinterpret_cast<uint4*>(d + (row0 + rr) * ld + col0 + c), make_uint4(w0, w1, w2, w3));
+                    }
+                    __syncwarp();
+                }
+            }
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 2) mbar_arrive_cluster(tempty0 + acc * 8);
+                else mbar_arrive(bar_tempty + acc * 8);
+            }
+        }
+    }
+
+    tcgen05_fence_before();
+    __syncthreads();
+    if constexpr (CG == 2) cluster_sync_all();
+    if (warp == 1) tmem_dealloc<CG>(tmem_base, 512);
+}
+
+}  // namespace avefp4
