@@ -35,7 +35,7 @@ EXPORTS = (
 # every symbol include/ave_dense.h declares
 DENSE_EXPORTS = (
     "ave_int8_quantize", "ave_int8_gemm", "ave_int8_gemm_gated", "ave_bf16_gemm_gated", "ave_bf16_gated_backward",
-    "ave_bf16_gated_backward_workspace_bytes", "ave_bf16_gemm_backward",
+    "ave_bf16_gated_backward_workspace_bytes", "ave_bf16_gemm_backward", "ave_bf16_gemm_backward_workspace_bytes",
 )
 
 
@@ -108,11 +108,13 @@ def load() -> ctypes.CDLL:
         L.ave_bf16_gemm_gated.restype = i32
         L.ave_bf16_gemm_gated.argtypes = [vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i64, vp, i64, i64, i64, i64, vp]
         L.ave_bf16_gated_backward_workspace_bytes.restype = i64
-        L.ave_bf16_gated_backward_workspace_bytes.argtypes = [i64, i64]
+        L.ave_bf16_gated_backward_workspace_bytes.argtypes = [i64, i64, i64, i32, i32]
         L.ave_bf16_gated_backward.restype = i32
         L.ave_bf16_gated_backward.argtypes = [vp, i64] * 6 + [i32, vp, i64, vp, vp, i64, vp, i64, i64, i64, i64, vp]
         L.ave_bf16_gemm_backward.restype = i32
-        L.ave_bf16_gemm_backward.argtypes = [vp, i64] * 5 + [i64, i64, i64, vp]
+        L.ave_bf16_gemm_backward.argtypes = [vp, i64] * 6 + [i64, i64, i64, vp]
+        L.ave_bf16_gemm_backward_workspace_bytes.restype = i64
+        L.ave_bf16_gemm_backward_workspace_bytes.argtypes = [i64, i64, i64, i32, i32]
         L.ave_fp4_set_trace.restype = i32
         L.ave_fp4_set_trace.argtypes = [vp, i64]
         _lib = L

@@ -87,19 +87,20 @@ def gemm_transposed_b_backward(dout: torch.Tensor, A: torch.Tensor, B: torch.Ten
     lda = _dense.matrix(A, "A", torch.bfloat16)
     m, k = A.shape
     dev = A.device
-    ldb = _dense.matrix(B, "B", torch.bfloat16, None, dev)
+    ldb = _dense.matrix(B, "B", torch.bfloat16, None, None, dev)
     n = B.shape[0]
     if B.shape[1] != k:
         raise ValueError(f"A and B must share K, got {k} and {B.shape[1]}.")
     _dense.multiple(n, "N", GROUP_N)
     _dense.multiple(k, "K", GROUP_K, positive=True)
-    ldo = _dense.matrix(dout, "dout", torch.bfloat16, (m, n), dev)
-    da = torch.empty((m, k), dtype=torch.bfloat16, device=dev) if need_da else None
-    db = torch.empty((n, k), dtype=torch.bfloat16, device=dev) if need_db else None
+    ldo = _dense.matrix(dout, "dout", torch.bfloat16, m, n, dev)
+    da = torch.empty(m, k, dtype=torch.bfloat16, device=dev) if need_da else None
+    db = torch.empty(n, k, dtype=torch.bfloat16, device=dev) if need_db else None
     if m and n:
         if need_da or need_db:
+            hold, workspace, need = _dense.workspace("ave_bf16_gemm_backward", dev, m, n, k, need_da, need_db)
             _dense.call("ave_bf16_gemm_backward", dev, dout.data_ptr(), ldo, A.data_ptr(), lda, B.data_ptr(), ldb,
-                        da.data_ptr() if need_da else None, k, db.data_ptr() if need_db else None, k, m, n, k)
+                        da.data_ptr() if need_da else None, k, db.data_ptr() if need_db else None, k, workspace, need, m, n, k)
     else:      # an empty sum
         for d in (da, db):
             if d is not None:

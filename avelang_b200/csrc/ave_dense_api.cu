@@ -89,67 +89,156 @@ struct Operand {
     int64_t ld;
 };
 
-// Columns of a tile: whole waves first.  A launch takes (waves) x (time of a tile), and the tile's time goes with its
-// columns plus a share that does not (hand-over, the A panel).
-int choose_block_n(int64_t cols, int64_t tile_rows, int64_t clusters, int step) {
-    int best = 256;
+// What a launch of the tile kernel is made of.
+struct DensePlan {
+    int cg;          // CTAs of a tile
+    int block_n;
+    int splits;      // ranges of K, of kb_split stages each (the last may be shorter)
+    int kb_split;
+    int a_rows, b_rows, kb_stage, stages;
+};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tile width, CTA pairs or single CTAs, and cuts of K: the smallest estimate of the launch's time, in SM clocks.
+//
+// A K block of 128 bytes per row takes a CTA the longest of: 2 block_n clocks of the tensor pipe (128 rows, 4 instructions);
+// 2 (a_rows + b_rows) to bring the operands from L2 (64 bytes a clock, what 256 x 256 tiles sustain on all SMs); 140 of issue;
+// and with one tile row, whose weights come from memory, the share of 3400 bytes a clock, at most 40 of them for one SM.  Work
+// comes in waves of all CTAs.  Cutting K into S ranges costs writing and reading S fp32 results (2600 bytes a clock) and
+// a launch.
+DensePlan plan_dense(int sms, int64_t m, int64_t cols, int64_t k_bytes, int segments, int batches, bool a_mn, bool b_mn,
+                     bool gated, bool may_split) {
+    DensePlan best{};
     int64_t best_cost = INT64_MAX;
-    for (int bn = 256; bn >= 64; bn -= step) {
-        const int64_t tiles = tile_rows * ((cols + bn - 1) / bn);
-        const int64_t cost = (tiles + clusters - 1) / clusters * (bn + 32);
-        if (cost < best_cost) {
-            best_cost = cost;
-            best = bn;
+    for (int cg = (m <= 128 ? 1 : 2); cg >= 1; --cg) {
+        const int64_t clusters = sms / cg;
+        const int64_t tile_rows = ceil_div(m, 128 * cg) * batches;
+        const int a_rows = (a_mn || m >= 128) ? 128 : static_cast<int>(ceil_div(m, 8) * 8);
+        const int step = cg == 2 ? 32 : gated ? 16 : 8;
+        for (int bn = 256; bn >= 32; bn -= step) {
+            const int b_rows = b_mn ? static_cast<int>(ceil_div(bn / cg, 64) * 64) : bn / cg;
+            const int64_t tiles = tile_rows * ceil_div(cols, bn);
+            int64_t clk = 2 * bn;
+            if (2 * (a_rows + b_rows) > clk) clk = 2 * (a_rows + b_rows);
+            if (clk < 140) clk = 140;
+            if (tile_rows == 1) {
+                const int64_t active = (tiles < clusters ? tiles : clusters) * cg;
+                const int64_t all = b_rows * 128 * active / 3400, one = b_rows * 128 / 40;
+                if (all > clk) clk = all;
+                if (one > clk) clk = one;
+            }
+            const int kbs = bn <= 128 ? 2 : 1;
+            const int64_t steps = ceil_div(k_bytes, 128 * kbs) * segments;
+            for (int64_t splits = 1; splits <= (may_split ? 8 : 1) && splits <= steps; ++splits) {
+                if (splits > 1 && tiles * (splits - 1) >= clusters) break;       // a wave is full without more of them
+                const int64_t kb_split = ceil_div(steps, splits);
+                const int64_t ranges = ceil_div(steps, kb_split);
+                int64_t cost = ceil_div(tiles * ranges, clusters) * (kb_split * kbs * clk + 400);
+                if (ranges > 1) cost += ranges * m * batches * cols * 8 / 2600 + 4000;
+                if (cost < best_cost) {
+                    best_cost = cost;
+                    best = DensePlan{cg, bn, static_cast<int>(ranges), static_cast<int>(kb_split), a_rows, b_rows, kbs, 0};
+                }
+            }
         }
     }
+    best.stages = DenseConfig<1>::stages(best.a_rows, best.b_rows, best.kb_stage);
     return best;
 }
 
-// m, n: result sizes (of one result); k: sum length of one segment.  a[1] / b[1]: second operand of two segments, two
-// results, or the second weight of the gated form.
+template <int OP>
+constexpr int64_t elem_bytes() { return OP == kOpInt8 ? 1 : 2; }
+
+// m, n: sizes of one result; k: sum length of one segment.  A plan depends on the sizes alone and takes a few microseconds
+// to find, as long as a small product runs: each host thread keeps the last ones it made.
+template <int OP, int EPI>
+DensePlan plan_for(const HostDevice& dev, int64_t m, int64_t n, int64_t k, int segments, int batches) {
+    struct Slot {
+        int64_t m, n, k;
+        int sms, segments, batches;
+        DensePlan plan;
+    };
+    constexpr int kSlots = 64;
+    thread_local Slot slots[kSlots] = {};
+    uint64_t h = (static_cast<uint64_t>(m) * 0x9E3779B97F4A7C15ull) ^ (static_cast<uint64_t>(n) * 0xC2B2AE3D27D4EB4Full) ^ static_cast<uint64_t>(k);
+    Slot& slot = slots[((h * 0xD6E8FEB86659FD93ull) >> 32) % kSlots];
+    if (slot.m != m || slot.n != n || slot.k != k || slot.sms != dev.sm_count || slot.segments != segments || slot.batches != batches) {
+        slot.plan = plan_dense(dev.sm_count, m, EPI == kDenseGated ? 2 * n : n, k * elem_bytes<OP>(), segments, batches, OP == kOpBf16Tn,
+                               OP == kOpBf16Nn || OP == kOpBf16Tn, EPI == kDenseGated, EPI == kDensePlain);
+        slot.m = m;
+        slot.n = n;
+        slot.k = k;
+        slot.sms = dev.sm_count;
+        slot.segments = segments;
+        slot.batches = batches;
+    }
+    return slot.plan;
+}
+
 template <int CG, int OP, int EPI>
-int launch_dense(const HostDevice& dev, const Operand (&a)[2], const Operand (&b)[2], int64_t m, int64_t n, int64_t k,
-                 DenseParams p, cudaStream_t stream) {
+int launch_dense_cg(const HostDevice& dev, const DensePlan& plan, const Operand (&a)[2], const Operand (&b)[2], int64_t m, int64_t n, int64_t k,
+                    DenseParams p, cudaStream_t stream) {
     using Cfg = DenseConfig<CG>;
     constexpr bool kAMn = (OP == kOpBf16Tn), kBMn = (OP == kOpBf16Nn || OP == kOpBf16Tn);
-    constexpr int kElem = (OP == kOpInt8) ? 1 : 2;
-    constexpr int kBlockK = 128 / kElem;
+    constexpr int64_t kElem = elem_bytes<OP>();
+    const int out_cols = (EPI == kDenseGated) ? plan.block_n / 2 : plan.block_n;
     p.m = static_cast<int>(m);
     p.n = static_cast<int>(n);
-    p.num_kb = static_cast<int>((k + kBlockK - 1) / kBlockK);
-    p.tiles_m = static_cast<int>((m + 128 * CG - 1) / (128 * CG));
-    const int64_t clusters = dev.sm_count / CG;
-    const int64_t cols = (EPI == kDenseGated) ? 2 * n : n;
-    p.block_n = choose_block_n(cols, int64_t(p.tiles_m) * p.batches, clusters, kBMn ? 64 * CG : (EPI == kDenseGated || CG == 2) ? 32 : 16);
-    const int out_cols = (EPI == kDenseGated) ? p.block_n / 2 : p.block_n;
-    p.tiles_n = static_cast<int>((n + out_cols - 1) / out_cols);
+    p.block_n = plan.block_n;
+    p.a_rows = plan.a_rows;
+    p.b_rows = plan.b_rows;
+    p.kb_stage = plan.kb_stage;
+    p.stages = plan.stages;
+    p.splits = plan.splits;
+    p.kb_split = plan.kb_split;
+    p.num_kb = static_cast<int>(ceil_div(k * kElem, 128 * plan.kb_stage));
+    p.tiles_m = static_cast<int>(ceil_div(m, 128 * CG));
+    p.tiles_n = static_cast<int>(ceil_div(n, out_cols));
     p.band = 8;
     p.status = dev.status;
-    p.pdl = 1;
 
     CUtensorMap ta[2], tb[2];
-    const int b_rows = (EPI == kDenseGated) ? out_cols : p.block_n / CG;
+    const int b_box = (EPI == kDenseGated) ? out_cols : plan.block_n / CG;
     for (int i = 0; i < 2; ++i) {
         int rc;
         if (kAMn) rc = host_encode_bytes(&ta[i], a[i].p, m * kElem, k, a[i].ld * kElem, 64, "A");
-        else rc = host_encode_bytes(&ta[i], a[i].p, k * kElem, m, a[i].ld * kElem, 128, "A");
+        else rc = host_encode_bytes(&ta[i], a[i].p, k * kElem, m, a[i].ld * kElem, p.a_rows, "A");
         if (rc) return rc;
         if (kBMn) rc = host_encode_bytes(&tb[i], b[i].p, n * kElem, k, b[i].ld * kElem, 64, "B");
-        else rc = host_encode_bytes(&tb[i], b[i].p, k * kElem, n, b[i].ld * kElem, b_rows, "B");
+        else rc = host_encode_bytes(&tb[i], b[i].p, k * kElem, n, b[i].ld * kElem, b_box, "B");
         if (rc) return rc;
     }
-    const int64_t tiles = int64_t(p.tiles_m) * p.batches * p.tiles_n;
-    Launch launch((tiles < clusters ? tiles : clusters) * CG, Cfg::kThreads, Cfg::kSmemBytes, CG, stream);
+    const int64_t items = int64_t(p.tiles_m) * p.batches * p.tiles_n * p.splits;
+    const int64_t clusters = dev.sm_count / CG;
+    Launch launch((items < clusters ? items : clusters) * CG, Cfg::kThreads, Cfg::kSmemBytes, CG, stream);
     AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gemm_dense_kernel<CG, OP, EPI>, ta[0], ta[1], tb[0], tb[1], p));
     return 0;
 }
 
+// a[1] / b[1]: second operand of two segments, two results, or the second weight of the gated form
 template <int OP, int EPI>
-int launch_dense_rows(const HostDevice& dev, const Operand (&a)[2], const Operand (&b)[2], int64_t m, int64_t n, int64_t k,
-                      const DenseParams& p, cudaStream_t stream) {
-    // up to 128 rows fill one CTA's tile: all SMs then take columns of their own instead of half a pair's empty rows
-    if (m <= 128) return launch_dense<1, OP, EPI>(dev, a, b, m, n, k, p, stream);
-    return launch_dense<2, OP, EPI>(dev, a, b, m, n, k, p, stream);
+int launch_dense(const HostDevice& dev, const DensePlan& plan, const Operand (&a)[2], const Operand (&b)[2], int64_t m, int64_t n, int64_t k,
+                 const DenseParams& p, cudaStream_t stream) {
+    if (plan.cg == 1) return launch_dense_cg<1, OP, EPI>(dev, plan, a, b, m, n, k, p, stream);
+    return launch_dense_cg<2, OP, EPI>(dev, plan, a, b, m, n, k, p, stream);
+}
+
+int64_t split_floats(const DensePlan& plan, int64_t rows, int64_t n) { return plan.splits > 1 ? plan.splits * rows * n : 0; }
+
+SplitSum split_sum(const DensePlan& plan, const float* partial, int64_t stride, void* d, int64_t ldd, int64_t rows, int64_t n) {
+    return SplitSum{partial, stride, static_cast<__nv_bfloat16*>(d), ldd, plan.splits > 1 ? rows * n / 8 : 0, static_cast<int>(n / 8), plan.splits};
+}
+
+int launch_sums(const HostDevice& dev, const SplitSums& sums, cudaStream_t stream) {
+    int64_t most = 0;
+    for (const SplitSum& s : sums.job) if (s.pieces > most) most = s.pieces;
+    if (most == 0) return 0;
+    int64_t grid = ceil_div(most, 256);
+    if (grid > int64_t(dev.sm_count) * 8) grid = int64_t(dev.sm_count) * 8;
+    Launch launch(grid, 256, 0, 1, stream);
+    AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, sum_splits_kernel, sums));
+    return 0;
 }
 
 DenseParams dense_params() {
@@ -161,14 +250,24 @@ DenseParams dense_params() {
 }
 
 // ------------------------------------------------------------------------------ a few tokens
-constexpr int64_t kStreamMaxM = 16;
+// Up to 8 rows go to the streaming kernel (its floor is the weights' bytes, and it reaches 90 to 99 % of it).  For 9 to 16 its
+// activations no longer fit L1 beside the ring, so large weights go to the tile kernel.  us, streaming / tile: int8 16 x 1024
+// x 8192 6.1 / 13.3, 16 x 4096 x 4096 8.0 / 8.9, 16 x 8192 x 8192 18.6 / 17.2, 16 x 28672 x 8192 48.6 / 44.5, gated bf16
+// 16 x 14336 x 8192 86 / 76.
+bool stream_rows(int64_t m, int64_t weight_bytes) { return m <= 8 || (m <= 16 && weight_bytes <= (int64_t(32) << 20)); }
 
-template <bool INT8, bool GATED, int ROWS>
-int launch_stream(const StreamParams& p, cudaStream_t stream) {
-    const int out = GATED ? ROWS / 2 : ROWS;
-    Launch launch((p.n + out - 1) / out, kStreamWarps * 32, 0, 1, stream);
-    if (p.m <= 8) AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gemm_stream_kernel<INT8, GATED, true, ROWS>, p));
-    else AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gemm_stream_kernel<INT8, GATED, false, ROWS>, p));
+
+template <bool INT8, bool GATED>
+int launch_stream(const HostDevice& dev, StreamParams p, cudaStream_t stream) {
+    const int64_t groups = (p.n + 7) / 8;
+    p.status = dev.status;
+    const bool m8 = p.m <= 8;
+    // The activations are read through what the ring leaves of L1: a third stage takes that down to some 30 KB.  It is worth 4 to
+    // 7 % for one token on a chip at 1.4 GHz under its power cap (nothing at 1.9), and costs 8 tokens of 8 KB 10 %.
+    p.stages = (m8 && static_cast<int64_t>(p.m) * p.k_bytes <= (24 << 10)) ? 3 : 2;
+    Launch launch(groups < dev.sm_count ? groups : dev.sm_count, kStreamThreads, m8 ? StreamConfig<true>::smem_bytes(p.stages) : StreamConfig<false>::smem_bytes(p.stages), 1, stream);
+    if (m8) AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gemm_stream_kernel<INT8, GATED, true>, p));
+    else AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gemm_stream_kernel<INT8, GATED, false>, p));
     return 0;
 }
 
@@ -181,7 +280,6 @@ StreamParams stream_params(const void* x, int64_t ldx_bytes, int64_t m, int64_t 
     p.n = static_cast<int>(n);
     p.k_bytes = static_cast<int>(k_bytes);
     p.act = act;
-    p.pdl = 1;
     p.d = static_cast<__nv_bfloat16*>(d);
     p.ldd = ldd;
     return p;
@@ -193,13 +291,13 @@ int launch_quantize(const void* x, int64_t rows, int64_t k, int64_t ldx, void* v
     Launch launch((rows + per_cta - 1) / per_cta, kInt8Threads, 0, 1, stream);
     AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, quantize_int8_kernel<NV, CTA_ROW>, static_cast<const __nv_bfloat16*>(x),
                                 static_cast<long long>(rows), static_cast<int>(k), static_cast<long long>(ldx), static_cast<int8_t*>(values),
-                                static_cast<long long>(ldv), static_cast<float*>(scales), 1));
+                                static_cast<long long>(ldv), static_cast<float*>(scales)));
     return 0;
 }
 
 template <int ACT>
 int launch_gated_backward(const HostDevice& dev, const void* dd, int64_t ld_dd, const void* gate, int64_t ld_gate, const void* up,
-                          int64_t ld_up, void* d_gate, void* d_up, int64_t m, int64_t f, cudaStream_t stream) {
+                          int64_t ld_up, void* d_gate, void* d_up, int64_t ld, int64_t m, int64_t f, cudaStream_t stream) {
     const int64_t pieces = m * (f / 8);
     const int64_t most = int64_t(dev.sm_count) * 8;
     int64_t grid = (pieces + 255) / 256;
@@ -208,7 +306,7 @@ int launch_gated_backward(const HostDevice& dev, const void* dd, int64_t ld_dd, 
     AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gated_backward_kernel<ACT>, static_cast<const __nv_bfloat16*>(dd), static_cast<long long>(ld_dd),
                                 static_cast<const __nv_bfloat16*>(gate), static_cast<long long>(ld_gate), static_cast<const __nv_bfloat16*>(up),
                                 static_cast<long long>(ld_up), static_cast<__nv_bfloat16*>(d_gate), static_cast<__nv_bfloat16*>(d_up),
-                                static_cast<long long>(m), static_cast<int>(f / 8), 1));
+                                static_cast<long long>(ld), static_cast<long long>(m), static_cast<int>(f / 8)));
     return 0;
 }
 
@@ -233,8 +331,20 @@ cudaError_t prepare_dense_kernels() {
     PREP(2, kOpInt8, kDenseGated)
     PREP(1, kOpBf16, kDenseGated)
     PREP(2, kOpBf16, kDenseGated)
+    PREP(1, kOpBf16Nn, kDensePlain)
     PREP(2, kOpBf16Nn, kDensePlain)
+    PREP(1, kOpBf16Tn, kDensePlain)
     PREP(2, kOpBf16Tn, kDensePlain)
+#undef PREP
+#define PREP(INT8, GATED, M8)                                                                                                          \
+    if ((e = cudaFuncSetAttribute(gemm_stream_kernel<INT8, GATED, M8>, cudaFuncAttributeMaxDynamicSharedMemorySize, StreamConfig<M8>::smem_bytes(StreamConfig<M8>::kMaxStages))) != cudaSuccess) \
+        return e;
+    PREP(true, false, true)
+    PREP(true, false, false)
+    PREP(true, true, true)
+    PREP(true, true, false)
+    PREP(false, true, true)
+    PREP(false, true, false)
 #undef PREP
     return cudaSuccess;
 }
@@ -294,14 +404,14 @@ int ave_int8_gemm(const void* a, int64_t lda, const void* a_scales, const void* 
     ldb = row_stride(n, k, ldb);
     ldd = row_stride(m, n, ldd);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (m <= kStreamMaxM) {
+    if (stream_rows(m, n * k)) {
         StreamParams p = stream_params(a, lda, m, n, k, activation, d_bf16, ldd);
         p.w[0] = static_cast<const uint8_t*>(b);
         p.ldw[0] = ldb;
         p.x_scale = static_cast<const float*>(a_scales);
         p.w_scale[0] = static_cast<const float*>(b_scales);
         p.bias = static_cast<const __nv_bfloat16*>(bias_bf16);
-        return n >= 16 * 4 * dev.sm_count ? launch_stream<true, false, 16>(p, s) : launch_stream<true, false, 8>(p, s);
+        return launch_stream<true, false>(dev, p, s);
     }
     DenseParams p = dense_params();
     p.a_scale = static_cast<const float*>(a_scales);
@@ -310,7 +420,7 @@ int ave_int8_gemm(const void* a, int64_t lda, const void* a_scales, const void* 
     p.act = activation;
     p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(d_bf16);
     p.ldd = ldd;
-    return launch_dense_rows<kOpInt8, kDenseScaled>(dev, {{a, lda}, {a, lda}}, {{b, ldb}, {b, ldb}}, m, n, k, p, s);
+    return launch_dense<kOpInt8, kDenseScaled>(dev, plan_for<kOpInt8, kDenseScaled>(dev, m, n, k, 1, 1), {{a, lda}, {a, lda}}, {{b, ldb}, {b, ldb}}, m, n, k, p, s);
 }
 
 int ave_int8_gemm_gated(const void* a, int64_t lda, const void* a_scales, const void* w_gate, int64_t ld_wg, const void* gate_scales,
@@ -337,7 +447,7 @@ int ave_int8_gemm_gated(const void* a, int64_t lda, const void* a_scales, const 
     ld_wu = row_stride(f, k, ld_wu);
     ldd = row_stride(m, f, ldd);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (m <= kStreamMaxM) {
+    if (stream_rows(m, 2 * f * k)) {
         StreamParams p = stream_params(a, lda, m, f, k, activation, d_bf16, ldd);
         p.w[0] = static_cast<const uint8_t*>(w_gate);
         p.w[1] = static_cast<const uint8_t*>(w_up);
@@ -346,7 +456,7 @@ int ave_int8_gemm_gated(const void* a, int64_t lda, const void* a_scales, const 
         p.x_scale = static_cast<const float*>(a_scales);
         p.w_scale[0] = static_cast<const float*>(gate_scales);
         p.w_scale[1] = static_cast<const float*>(up_scales);
-        return launch_stream<true, true, 16>(p, s);
+        return launch_stream<true, true>(dev, p, s);
     }
     DenseParams p = dense_params();
     p.a_scale = static_cast<const float*>(a_scales);
@@ -355,7 +465,7 @@ int ave_int8_gemm_gated(const void* a, int64_t lda, const void* a_scales, const 
     p.act = activation;
     p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(d_bf16);
     p.ldd = ldd;
-    return launch_dense_rows<kOpInt8, kDenseGated>(dev, {{a, lda}, {a, lda}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, k, p, s);
+    return launch_dense<kOpInt8, kDenseGated>(dev, plan_for<kOpInt8, kDenseGated>(dev, m, f, k, 1, 1), {{a, lda}, {a, lda}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, k, p, s);
 }
 
 int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t ld_wg, const void* w_up, int64_t ld_wu, int activation,
@@ -385,7 +495,7 @@ int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t 
     ld_gate = row_stride(m, f, ld_gate);
     ld_up = row_stride(m, f, ld_up);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (m <= kStreamMaxM) {
+    if (stream_rows(m, 4 * f * h)) {
         StreamParams p = stream_params(x, ldx * 2, m, f, h * 2, activation, d_bf16, ldd);
         p.w[0] = static_cast<const uint8_t*>(w_gate);
         p.w[1] = static_cast<const uint8_t*>(w_up);
@@ -395,7 +505,7 @@ int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t 
         p.up = static_cast<__nv_bfloat16*>(up_bf16);
         p.ld_gate = ld_gate;
         p.ld_up = ld_up;
-        return launch_stream<false, true, 16>(p, s);
+        return launch_stream<false, true>(dev, p, s);
     }
     DenseParams p = dense_params();
     p.act = activation;
@@ -405,14 +515,72 @@ int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t 
     p.up = static_cast<__nv_bfloat16*>(up_bf16);
     p.ld_gate = ld_gate;
     p.ld_up = ld_up;
-    return launch_dense_rows<kOpBf16, kDenseGated>(dev, {{x, ldx}, {x, ldx}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, h, p, s);
+    return launch_dense<kOpBf16, kDenseGated>(dev, plan_for<kOpBf16, kDenseGated>(dev, m, f, h, 1, 1), {{x, ldx}, {x, ldx}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, h, p, s);
 }
 
-static int64_t gated_backward_half(int64_t m, int64_t f) { return (m * f * 2 + 255) / 256 * 256; }
+}  // extern "C"
 
-int64_t ave_bf16_gated_backward_workspace_bytes(int64_t m, int64_t f) {
-    if (!sizes_ok(m, f, 0)) return fail("ave_bf16_gated_backward_workspace_bytes: size out of range");
-    return 2 * gated_backward_half(m, f);
+namespace {
+
+// Workspace of the gated block's backward pass: dG and dU with rows padded to whole 128-byte lines (a box row of a TMA load
+// then touches one line), and what cuts of K in either product need.
+struct GatedBackwardPlan {
+    DensePlan dx, dw;
+    int64_t ld, half, dx_floats, dw_floats;
+    int64_t bytes() const { return 2 * half + 4 * (dx_floats + dw_floats); }
+};
+
+GatedBackwardPlan plan_gated_backward(const HostDevice& dev, int64_t m, int64_t f, int64_t h, bool want_x, bool want_w) {
+    GatedBackwardPlan p{};
+    p.ld = ceil_div(f, 64) * 64;
+    p.half = ceil_div(m * p.ld * 2, 256) * 256;
+    if (want_x) {
+        p.dx = plan_for<kOpBf16Nn, kDensePlain>(dev, m, h, f, 2, 1);
+        p.dx_floats = split_floats(p.dx, m, h);
+    }
+    if (want_w) {
+        p.dw = plan_for<kOpBf16Tn, kDensePlain>(dev, f, h, m, 1, 2);
+        p.dw_floats = split_floats(p.dw, 2 * f, h);
+    }
+    return p;
+}
+
+struct ProductBackwardPlan {
+    DensePlan da, db;
+    int64_t da_floats, db_floats;
+    int64_t bytes() const { return 4 * (da_floats + db_floats); }
+};
+
+ProductBackwardPlan plan_product_backward(const HostDevice& dev, int64_t m, int64_t n, int64_t k, bool want_a, bool want_b) {
+    ProductBackwardPlan p{};
+    if (want_a) {
+        p.da = plan_for<kOpBf16Nn, kDensePlain>(dev, m, k, n, 1, 1);
+        p.da_floats = split_floats(p.da, m, k);
+    }
+    if (want_b) {
+        p.db = plan_for<kOpBf16Tn, kDensePlain>(dev, n, k, m, 1, 1);
+        p.db_floats = split_floats(p.db, n, k);
+    }
+    return p;
+}
+
+int check_workspace(const char* fn, const void* workspace, int64_t have, int64_t need) {
+    if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || have < need))
+        return fail("%s: the workspace must be 256-byte aligned and hold %lld bytes", fn, static_cast<long long>(need));
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t ave_bf16_gated_backward_workspace_bytes(int64_t m, int64_t f, int64_t h, int want_dx, int want_dw) {
+    HostDevice dev;
+    if (!sizes_ok(m, f, h)) return fail("ave_bf16_gated_backward_workspace_bytes: size out of range");
+    if (m == 0 || f == 0 || h == 0 || !(want_dx || want_dw)) return 0;
+    const int rc = host_device(&dev);
+    if (rc) return rc < 0 ? rc : -rc;
+    return plan_gated_backward(dev, m, f, h, want_dx != 0, want_dw != 0).bytes();
 }
 
 int ave_bf16_gated_backward(const void* dd, int64_t ld_dd, const void* x, int64_t ldx, const void* w_gate, int64_t ld_wg,
@@ -448,31 +616,37 @@ int ave_bf16_gated_backward(const void* dd, int64_t ld_dd, const void* x, int64_
     CHECK(check_matrix(fn, "gate", gate, m, f, ld_gate, 2));
     CHECK(check_matrix(fn, "up", up, m, f, ld_up, 2));
     if (!want_x && !want_w) return 0;
-    const int64_t half = gated_backward_half(m, f);
-    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || workspace_bytes < 2 * half)
-        return fail("%s: the workspace must be 256-byte aligned and hold %lld bytes", fn, static_cast<long long>(2 * half));
     CHECK(host_device(&dev));
+    const GatedBackwardPlan plan = plan_gated_backward(dev, m, f, h, want_x, want_w);
+    CHECK(check_workspace(fn, workspace, workspace_bytes, plan.bytes()));
     ld_dd = row_stride(m, f, ld_dd);
     ldx = row_stride(m, h, ldx);
     ld_wg = row_stride(f, h, ld_wg);
     ld_wu = row_stride(f, h, ld_wu);
     ld_gate = row_stride(m, f, ld_gate);
     ld_up = row_stride(m, f, ld_up);
+    const int64_t ld = plan.ld;
     void* d_gate = workspace;
-    void* d_up = static_cast<uint8_t*>(workspace) + half;
+    void* d_up = static_cast<uint8_t*>(workspace) + plan.half;
+    float* dx_partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 2 * plan.half);
+    float* dw_partial = dx_partial + plan.dx_floats;
+    SplitSums sums{};
     switch (activation) {
-        case AVE_FP4_ACT_RELU: CHECK(launch_gated_backward<AVE_FP4_ACT_RELU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
-        case AVE_FP4_ACT_GELU: CHECK(launch_gated_backward<AVE_FP4_ACT_GELU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
-        case AVE_FP4_ACT_GELU_TANH: CHECK(launch_gated_backward<AVE_FP4_ACT_GELU_TANH>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
-        case AVE_FP4_ACT_SILU: CHECK(launch_gated_backward<AVE_FP4_ACT_SILU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
-        default: CHECK(launch_gated_backward<AVE_FP4_ACT_NONE>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, m, f, s)); break;
+        case AVE_FP4_ACT_RELU: CHECK(launch_gated_backward<AVE_FP4_ACT_RELU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, ld, m, f, s)); break;
+        case AVE_FP4_ACT_GELU: CHECK(launch_gated_backward<AVE_FP4_ACT_GELU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, ld, m, f, s)); break;
+        case AVE_FP4_ACT_GELU_TANH: CHECK(launch_gated_backward<AVE_FP4_ACT_GELU_TANH>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, ld, m, f, s)); break;
+        case AVE_FP4_ACT_SILU: CHECK(launch_gated_backward<AVE_FP4_ACT_SILU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, ld, m, f, s)); break;
+        default: CHECK(launch_gated_backward<AVE_FP4_ACT_NONE>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, ld, m, f, s)); break;
     }
     if (want_x) {
         DenseParams p = dense_params();
         p.segments = 2;
         p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(dx);
         p.ldd = row_stride(m, h, ld_dx);
-        CHECK((launch_dense<2, kOpBf16Nn, kDensePlain>(dev, {{d_gate, f}, {d_up, f}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, h, f, p, s)));
+        p.partial = dx_partial;
+        p.trigger_late = want_w;
+        CHECK((launch_dense<kOpBf16Nn, kDensePlain>(dev, plan.dx, {{d_gate, ld}, {d_up, ld}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, h, f, p, s)));
+        sums.job[0] = split_sum(plan.dx, dx_partial, m * h, dx, p.ldd, m, h);
     }
     if (want_w) {
         DenseParams p = dense_params();
@@ -480,13 +654,27 @@ int ave_bf16_gated_backward(const void* dd, int64_t ld_dd, const void* x, int64_
         p.d[0] = static_cast<__nv_bfloat16*>(dw_gate);
         p.d[1] = static_cast<__nv_bfloat16*>(dw_up);
         p.ldd = row_stride(f, h, ld_dw);
-        CHECK((launch_dense<2, kOpBf16Tn, kDensePlain>(dev, {{d_gate, f}, {d_up, f}}, {{x, ldx}, {x, ldx}}, f, h, m, p, s)));
+        p.partial = dw_partial;
+        p.wait_late = want_x;
+        CHECK((launch_dense<kOpBf16Tn, kDensePlain>(dev, plan.dw, {{d_gate, ld}, {d_up, ld}}, {{x, ldx}, {x, ldx}}, f, h, m, p, s)));
+        sums.job[1] = split_sum(plan.dw, dw_partial, 2 * f * h, dw_gate, p.ldd, f, h);
+        sums.job[2] = split_sum(plan.dw, dw_partial + f * h, 2 * f * h, dw_up, p.ldd, f, h);
     }
-    return 0;
+    return launch_sums(dev, sums, s);
+}
+
+int64_t ave_bf16_gemm_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int want_da, int want_db) {
+    HostDevice dev;
+    if (!sizes_ok(m, n, k)) return fail("ave_bf16_gemm_backward_workspace_bytes: size out of range");
+    if (m == 0 || n == 0 || k == 0 || !(want_da || want_db)) return 0;
+    const int rc = host_device(&dev);
+    if (rc) return rc < 0 ? rc : -rc;
+    return plan_product_backward(dev, m, n, k, want_da != 0, want_db != 0).bytes();
 }
 
 int ave_bf16_gemm_backward(const void* dd, int64_t ld_dd, const void* a, int64_t lda, const void* b, int64_t ldb, void* da,
-                           int64_t ld_da, void* db, int64_t ld_db, int64_t m, int64_t n, int64_t k, void* stream) {
+                           int64_t ld_da, void* db, int64_t ld_db, void* workspace, int64_t workspace_bytes, int64_t m, int64_t n, int64_t k,
+                           void* stream) {
     static const char* fn = "ave_bf16_gemm_backward";
     HostDevice dev;
     if (!sizes_ok(m, n, k)) return fail("%s: size out of range", fn);
@@ -507,19 +695,30 @@ int ave_bf16_gemm_backward(const void* dd, int64_t ld_dd, const void* a, int64_t
     ld_dd = row_stride(m, n, ld_dd);
     lda = row_stride(m, k, lda);
     ldb = row_stride(n, k, ldb);
+    const ProductBackwardPlan plan = plan_product_backward(dev, m, n, k, da != nullptr, db != nullptr);
+    CHECK(check_workspace(fn, workspace, workspace_bytes, plan.bytes()));
+    float* da_partial = static_cast<float*>(workspace);
+    float* db_partial = da_partial + plan.da_floats;
+    SplitSums sums{};
     if (da != nullptr) {
         DenseParams p = dense_params();
         p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(da);
         p.ldd = row_stride(m, k, ld_da);
-        CHECK((launch_dense<2, kOpBf16Nn, kDensePlain>(dev, {{dd, ld_dd}, {dd, ld_dd}}, {{b, ldb}, {b, ldb}}, m, k, n, p, s)));
+        p.partial = da_partial;
+        p.trigger_late = db != nullptr;
+        CHECK((launch_dense<kOpBf16Nn, kDensePlain>(dev, plan.da, {{dd, ld_dd}, {dd, ld_dd}}, {{b, ldb}, {b, ldb}}, m, k, n, p, s)));
+        sums.job[0] = split_sum(plan.da, da_partial, m * k, da, p.ldd, m, k);
     }
     if (db != nullptr) {
         DenseParams p = dense_params();
         p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(db);
         p.ldd = row_stride(n, k, ld_db);
-        CHECK((launch_dense<2, kOpBf16Tn, kDensePlain>(dev, {{dd, ld_dd}, {dd, ld_dd}}, {{a, lda}, {a, lda}}, n, k, m, p, s)));
+        p.partial = db_partial;
+        p.wait_late = da != nullptr;
+        CHECK((launch_dense<kOpBf16Tn, kDensePlain>(dev, plan.db, {{dd, ld_dd}, {dd, ld_dd}}, {{a, lda}, {a, lda}}, n, k, m, p, s)));
+        sums.job[1] = split_sum(plan.db, db_partial, n * k, db, p.ldd, n, k);
     }
-    return 0;
+    return launch_sums(dev, sums, s);
 }
 
 }  // extern "C"

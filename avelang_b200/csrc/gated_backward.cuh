@@ -27,11 +27,9 @@ template <int ACT>
 __global__ void __launch_bounds__(256)
 gated_backward_kernel(const __nv_bfloat16* __restrict__ dout, long long ld_dout, const __nv_bfloat16* __restrict__ gate, long long ld_gate,
                       const __nv_bfloat16* __restrict__ up, long long ld_up, __nv_bfloat16* __restrict__ d_gate,
-                      __nv_bfloat16* __restrict__ d_up, long long rows, int f8, int pdl) {
-    if (pdl) {
-        pdl_launch_dependents();
-        pdl_wait_prior_grid();
-    }
+                      __nv_bfloat16* __restrict__ d_up, long long ld, long long rows, int f8) {
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
     const long long total = rows * f8;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
         const long long r = i / f8;
@@ -44,8 +42,8 @@ gated_backward_kernel(const __nv_bfloat16* __restrict__ dout, long long ld_dout,
         gated_backward_pair<ACT>(d.y, g.y, u.y, dg.y, du.y);
         gated_backward_pair<ACT>(d.z, g.z, u.z, dg.z, du.z);
         gated_backward_pair<ACT>(d.w, g.w, u.w, dg.w, du.w);
-        reinterpret_cast<uint4*>(d_gate)[i] = dg;
-        reinterpret_cast<uint4*>(d_up)[i] = du;
+        *reinterpret_cast<uint4*>(d_gate + r * ld + c) = dg;
+        *reinterpret_cast<uint4*>(d_up + r * ld + c) = du;
     }
 }
 

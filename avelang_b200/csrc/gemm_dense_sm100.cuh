@@ -17,7 +17,7 @@
 // in one thread's TMEM lane.  With CTA pairs this takes no extra load: each CTA supplies half of the B tile, one of
 // them from Wg, the other from Wu.
 //
-// Structure: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue; a ring of shared-memory stages of 128 bytes of
+// Structure: warps 0 and 2 TMA producers, warp 1 MMA issuer, warps 3-10 epilogue; a ring of shared-memory stages of 128 bytes of
 // K per row (128-byte swizzle); two accumulators of up to 256 columns in TMEM, so a tile's epilogue runs under the next
 // tile's main loop.  The tile is 128 rows per CTA by `block_n` columns, and block_n is a run-time value: the number of
 // columns goes into the instruction descriptor, so the host picks it for whole waves (see choose_block_n).
@@ -38,18 +38,28 @@ enum DenseEpilogue : int { kDensePlain = 0, kDenseScaled = 1, kDenseGated = 2 };
 struct DenseParams {
     long long ldd, ld_gate, ld_up;   // row strides in elements
     int m, n;                        // rows and columns of one result (gated: n = F)
-    int num_kb;                      // K blocks of one segment (64 bf16 or 128 int8 elements of K each)
+    int num_kb;                      // stages of K of one segment
+    int kb_stage;                    // K blocks of 128 bytes per row (64 bf16 or 128 int8 elements) in a stage: 1 or 2
     int segments;                    // 2: C = A0 B0 + A1 B1, two operand pairs of the same sizes
+    int kb_split;                    // stages of K in a range
+    int splits;                      // > 1 (plain epilogue): K is cut into that many ranges whose fp32 sums go to `partial`,
+                                     // [split][result][m][n], and sum_splits_kernel adds them up
     int batches;                     // 2: two results, C0 from A0 and C1 from A1, B shared; tile rows of C1 follow those of C0
     int tiles_m, tiles_n;            // tiles of one result
-    int block_n;                     // accumulator columns of a tile
+    int block_n;                     // columns of a tile, a multiple of 8 (one CTA) or 32 (pair)
+    int b_rows;                      // rows of B in a K block: block_n per CTA, or for an MN-major B the whole boxes of 64 that hold them
+    int stages;                      // stages of the ring that fit with this block_n
+    int a_rows;                      // rows of A in a K block: 128, or with fewer than that in all, those, to a multiple of 8
     int band;                        // tile rows per band of the schedule
     __nv_bfloat16* d[2];
+    float* partial;
     const float* a_scale;            // one per row of A
     const float* b_scale[2];         // one per row of B; gated: of Wg and Wu
     const __nv_bfloat16* bias;
     int act;
-    int pdl;                         // launched with programmatic stream serialisation
+    int wait_late;                   // the previous kernel in the stream writes nothing that this one reads or writes: run beside
+                                     // its tail and wait for it (so that whoever waits for this one has waited for both) at the end
+    int trigger_late;                // let the next kernel start only once the previous one has finished (the next is wait_late)
     __nv_bfloat16* gate;             // gated: where to keep G and U, or nullptr
     __nv_bfloat16* up;
     int* status;
@@ -57,21 +67,37 @@ struct DenseParams {
 
 template <int CG>
 struct DenseConfig {
-    static constexpr int kMaxN = 256;
-    static constexpr int kABytes = 128 * 128;
-    static constexpr int kBBytes = kMaxN / CG * 128;
-    static constexpr int kStages = (CG == 2) ? 6 : 4;
+    static constexpr int kRingBytes = 192 * 1024;        // stages of kb_stage * (a_rows + b_rows) * 128 bytes
+    static constexpr int kMaxStages = 16;
     static constexpr int kEpiWarps = 8;
     static constexpr int kEpiBufBytes = 32 * 128;
-    static constexpr int kOffA = 0;
-    static constexpr int kOffB = kStages * kABytes;
-    static constexpr int kOffEpi = kOffB + kStages * kBBytes;
+    static constexpr int kOffEpi = kRingBytes;
     static constexpr int kOffBar = kOffEpi + kEpiWarps * kEpiBufBytes;
-    static constexpr int kOffTmemPtr = kOffBar + (2 * kStages + 4) * 8;
+    static constexpr int kOffTmemPtr = kOffBar + (2 * kMaxStages + 4) * 8;
     static constexpr int kSmemBytes = kOffTmemPtr + 16 + 1024;
-    static constexpr int kThreads = 64 + 32 * kEpiWarps;
+    static constexpr int kThreads = 96 + 32 * kEpiWarps;
+    static constexpr int stages(int a_rows, int b_rows, int kb_stage) {
+        const int n = kRingBytes / (kb_stage * (a_rows + b_rows) * 128);
+        return n < kMaxStages ? n : kMaxStages;
+    }
     static_assert(kSmemBytes <= 232448, "shared memory budget");
 };
+
+// Tiled load with an L2 policy chosen at run time.
+template <int CG>
+__device__ __forceinline__ void tma_load(uint32_t dst, const void* tmap, uint32_t bar, int x, int y, uint64_t policy) {
+    if constexpr (CG == 1) {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+            ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y), "l"(policy)
+            : "memory");
+    } else {
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;"
+            ::"r"(dst), "l"(tmap), "r"(bar), "r"(x), "r"(y), "l"(policy)
+            : "memory");
+    }
+}
 
 // Instruction descriptor of kind::f16 / kind::i8: bits 4-5 accumulator (1 fp32, 2 int32), 7-9 / 10-12 operand formats
 // (kind::f16: 1 = bf16; kind::i8: 1 = signed), 15 / 16 A / B MN-major, 17-22 N >> 3, 24-28 M >> 4.
@@ -98,9 +124,11 @@ __device__ __forceinline__ void mma_int8(uint32_t d_tmem, uint64_t adesc, uint64
     }
 }
 
-// Tile number -> (tile row, tile column): bands of `band` tile rows, rows fastest inside a band, so that the CTAs
-// running at the same time share a few A panels and a few B panels in L2.
-__device__ __forceinline__ void dense_tile(int t, int rows, int cols, int band, int& tm, int& tn) {
+// Work item -> (tile row, tile column, K range): ranges slowest; bands of `band` tile rows, rows fastest inside a band, so that
+// the CTAs running at the same time share a few A panels and a few B panels in L2.
+__device__ __forceinline__ void dense_tile(int t, int rows, int cols, int band, int& tm, int& tn, int& split) {
+    split = 0;
+    for (const int one = rows * cols; t >= one; t -= one) ++split;       // a few ranges at most
     const int per_band = band * cols;
     const int g = t / per_band;
     const int first = g * band;
@@ -148,11 +176,10 @@ __device__ __forceinline__ void dense_convert(const uint32_t (&v)[32], const uin
 }
 
 template <int CG, int OP, int EPI>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(352, 1)
 gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constant__ CUtensorMap tm_a1,
                   const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1, const DenseParams p) {
     using Cfg = DenseConfig<CG>;
-    constexpr int STAGES = Cfg::kStages;
     constexpr bool kInt8 = (OP == kOpInt8);
     constexpr bool kAMn = (OP == kOpBf16Tn);
     constexpr bool kBMn = (OP == kOpBf16Nn || OP == kOpBf16Tn);
@@ -169,14 +196,19 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     const int cluster_id = blockIdx.x / CG;
     const int num_clusters = gridDim.x / CG;
     const int tile_rows = p.tiles_m * p.batches;
-    const int num_tiles = tile_rows * p.tiles_n;
-    const int num_kb = p.num_kb * p.segments;
-    const int bn_cta = p.block_n / CG;                            // rows of B that one CTA loads
+    const int num_tiles = tile_rows * p.tiles_n * p.splits;
+    const int all_kb = p.num_kb * p.segments;
+    const int stages = p.stages;
+    const int bn_cta = p.block_n / CG;                            // columns of the tile whose B one CTA loads
+    const int b_bytes = p.b_rows * 128;                           // whole 1 KB swizzle groups
+    const int a_bytes = p.a_rows * 128;
+    const int kbs = p.kb_stage;
+    const uint32_t ring_b = smem_base + stages * kbs * a_bytes;
     const int out_cols = kGated ? p.block_n / 2 : p.block_n;      // result columns of a tile
 
     const uint32_t bar_full = smem_base + Cfg::kOffBar;
-    const uint32_t bar_empty = bar_full + STAGES * 8;
-    const uint32_t bar_tfull = bar_empty + STAGES * 8;
+    const uint32_t bar_empty = bar_full + Cfg::kMaxStages * 8;
+    const uint32_t bar_tfull = bar_empty + Cfg::kMaxStages * 8;
     const uint32_t bar_tempty = bar_tfull + 2 * 8;
     const uint32_t tmem_ptr_smem = smem_base + Cfg::kOffTmemPtr;
     volatile uint32_t* tmem_ptr_gen = reinterpret_cast<volatile uint32_t*>(smem_gen + Cfg::kOffTmemPtr);
@@ -186,8 +218,8 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
         prefetch_tensormap(&tm_b0);
         prefetch_tensormap(&tm_a1);
         prefetch_tensormap(&tm_b1);
-        for (int s = 0; s < STAGES; ++s) {
-            mbar_init(bar_full + s * 8, 1);
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(bar_full + s * 8, 2);      // both producers of the leader
             mbar_init(bar_empty + s * 8, 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -206,77 +238,92 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     tcgen05_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_gen, 0);
 
-    if (warp == 0) {
-        // ------------------------------------------------------------ TMA producer
+    if (warp == 0 || warp == 2) {
+        // ------------------------------------------------------- TMA producers: warp 0 loads A, warp 2 loads B
+        // Each walks the whole schedule; with one warp for both, the issue loop and not the copies set the pace of narrow tiles.
+        const bool for_a = (warp == 0);
         const bool issuer = elect_one_sync();
-        if (p.pdl) {
-            if (issuer) pdl_launch_dependents();
-            pdl_wait_prior_grid();       // operands may come from the previous kernel
-        }
-        const uint32_t full0 = (CG == 2) ? mapa_shared(bar_full, 0) : bar_full;
-        const uint32_t tx_bytes = static_cast<uint32_t>(CG * (Cfg::kABytes + bn_cta * 128));
-        int stage = 0;
+        if (issuer && !p.trigger_late) pdl_launch_dependents();
+        if (!p.wait_late) pdl_wait_prior_grid();       // operands may come from the previous kernel
+        if (issuer && p.trigger_late) pdl_launch_dependents();
+        // operands that other CTAs read as well stay in L2; with a single tile row B passes through once
+        const uint64_t policy = (!for_a && tile_rows == 1) ? kL2EvictFirst : kL2EvictLast;
+        const uint32_t bytes = static_cast<uint32_t>(for_a ? a_bytes : b_bytes);
+        const uint32_t dst0 = for_a ? smem_base : ring_b;
+        const uint32_t peer = (CG == 2) ? mapa_shared(bar_full, 0) - bar_full : 0u;   // the leader's barriers count both CTAs' bytes
+        const uint32_t bar_end = bar_full + stages * 8;
+        uint32_t dst = dst0, full = bar_full, empty = bar_empty;
         uint32_t phase = 0;
         bool ok = true;
         for (int t = cluster_id; t < num_tiles && ok; t += num_clusters) {
-            int tm, tn;
-            dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn);
+            int tm, tn, split;
+            dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn, split);
             const bool second = tm >= p.tiles_m;                  // tile of the second result
             const int row_a = ((second ? tm - p.tiles_m : tm) * CG + rank) * 128;
             const int row_b = tn * out_cols + (kGated ? 0 : rank * bn_cta);
-            int seg = 0, kb = 0;
-            for (int i = 0; i < num_kb; ++i) {
-                if (!mbar_wait(bar_empty + stage * 8, phase ^ 1u)) {
-                    if (issuer) atomicCAS(p.status, 0, 101);
-                    ok = false;
-                    break;
-                }
-                if (issuer) {
-                    const uint32_t full = full0 + stage * 8;
-                    const uint32_t sa = smem_base + Cfg::kOffA + stage * Cfg::kABytes;
-                    const uint32_t sb = smem_base + Cfg::kOffB + stage * Cfg::kBBytes;
-                    const CUtensorMap* ta = (second || seg) ? &tm_a1 : &tm_a0;
-                    const CUtensorMap* tb = seg ? &tm_b1 : &tm_b0;
-                    if (is_leader) mbar_arrive_expect_tx(bar_full + stage * 8, tx_bytes);
-                    if constexpr (kAMn) {
-                        tma_load_2d<CG, 2>(sa, ta, full, row_a * 2, kb * 64);
-                        tma_load_2d<CG, 2>(sa + 8192, ta, full, row_a * 2 + 128, kb * 64);
-                    } else {
-                        tma_load_2d<CG, 2>(sa, ta, full, kb * 128, row_a);
+            int i = split * p.kb_split;
+            const int end = min(i + p.kb_split, all_kb);
+            int seg = (i >= p.num_kb) ? 1 : 0;
+            for (int kb = i - seg * p.num_kb; i < end; ++i, ++kb) {
+                    if (kb == p.num_kb) { kb = 0; seg = 1; }
+                    const CUtensorMap* map = for_a ? ((second || seg) ? &tm_a1 : &tm_a0)
+                                                   : ((seg || (kGated && CG == 2 && rank)) ? &tm_b1 : &tm_b0);
+                    if (!mbar_wait(empty, phase ^ 1u)) {
+                        if (issuer) atomicCAS(p.status, 0, 101);
+                        ok = false;
+                        break;
                     }
-                    if constexpr (kBMn) {
-                        for (int c = 0; c < bn_cta; c += 64)
-                            tma_load_2d<CG, 2>(sb + c * 128, tb, full, (row_b + c) * 2, kb * 64);
-                    } else if constexpr (kGated && CG == 2) {
-                        tma_load_2d<CG, 2>(sb, rank ? &tm_b1 : &tm_b0, full, kb * 128, row_b);
-                    } else if constexpr (kGated) {
-                        tma_load_2d<CG, 2>(sb, &tm_b0, full, kb * 128, row_b);
-                        tma_load_2d<CG, 2>(sb + out_cols * 128, &tm_b1, full, kb * 128, row_b);
-                    } else {
-                        tma_load_2d<CG, 2>(sb, tb, full, kb * 128, row_b);
+                    if (issuer) {
+                        if (is_leader) mbar_arrive_expect_tx(full, CG * kbs * bytes);
+                        const uint32_t bar = full + peer;
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            if (u == kbs) break;
+                            const int k = kb * kbs + u;             // past the end of K a load brings zeros
+                            const uint32_t to = dst + u * bytes;
+                            if (for_a) {
+                                if constexpr (kAMn) {
+                                    tma_load<CG>(to, map, bar, row_a * 2, k * 64, policy);
+                                    tma_load<CG>(to + 8192, map, bar, row_a * 2 + 128, k * 64, policy);
+                                } else {
+                                    tma_load<CG>(to, map, bar, k * 128, row_a, policy);
+                                }
+                            } else if constexpr (kBMn) {
+#pragma unroll
+                                for (int c = 0; c < 256 / CG; c += 64)
+                                    if (c < bn_cta) tma_load<CG>(to + c * 128, map, bar, (row_b + c) * 2, k * 64, policy);
+                            } else {
+                                tma_load<CG>(to, map, bar, k * 128, row_b, policy);
+                                if constexpr (kGated && CG == 1) tma_load<CG>(to + out_cols * 128, &tm_b1, bar, k * 128, row_b, policy);
+                            }
+                        }
                     }
-                }
-                if (++kb == p.num_kb) { kb = 0; ++seg; }
-                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    dst += kbs * bytes;
+                    full += 8;
+                    empty += 8;
+                    if (full == bar_end) { dst = dst0; full = bar_full; empty = bar_empty; phase ^= 1u; }
             }
         }
-        if (ok) {
-            // wait until every filled stage has been consumed: no copy or signal is outstanding when the CTA exits
-            for (int i = 0; i < STAGES; ++i) {
-                if (!mbar_wait(bar_empty + stage * 8, phase ^ 1u)) {
-                    if (issuer) atomicCAS(p.status, 0, 101);
-                    break;
-                }
-                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        // wait until every filled stage has been consumed: no copy or signal is outstanding when the CTA exits
+        for (int i = 0; i < stages && ok; ++i) {
+            if (!mbar_wait(empty, phase ^ 1u)) {
+                if (issuer) atomicCAS(p.status, 0, 101);
+                ok = false;
             }
+            full += 8;
+            empty += 8;
+            if (full == bar_end) { full = bar_full; empty = bar_empty; phase ^= 1u; }
         }
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------- MMA issuer
         if (is_leader) {
             const bool issuer = elect_one_sync();
-            const uint32_t idesc = make_idesc_dense(kInt8, kAMn, kBMn, 128 * CG, p.block_n);
-            int stage = 0;
+            // The instruction's columns come in 16s.  Where the tile has 8 fewer it reads on into whatever follows in the ring,
+            // as it does for rows of A that are not there: that reaches accumulator columns past the tile's last, which nobody uses.
+            const uint32_t idesc = make_idesc_dense(kInt8, kAMn, kBMn, 128 * CG, (p.block_n + 15) / 16 * 16);
+            const uint32_t bar_end = bar_full + stages * 8;
+            uint32_t sa = smem_base, sb = ring_b, full = bar_full, empty = bar_empty;
             uint32_t phase = 0;
             int tile_iter = 0;
             bool ok = true;
@@ -290,31 +337,41 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
                 }
                 tcgen05_fence_after();
                 const uint32_t d_tmem = tmem_base + acc * 256;
-                for (int i = 0; i < num_kb; ++i) {
-                    if (!mbar_wait(bar_full + stage * 8, phase)) {
+                int tm, tn, split;
+                dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn, split);
+                const int steps = min(p.kb_split, all_kb - split * p.kb_split);
+                for (int i = 0; i < steps; ++i) {
+                    if (!mbar_wait(full, phase)) {
                         if (issuer) atomicCAS(p.status, 0, 102);
                         ok = false;
                         break;
                     }
                     tcgen05_fence_after();
-                    const uint32_t sa = smem_base + Cfg::kOffA + stage * Cfg::kABytes;
-                    const uint32_t sb = smem_base + Cfg::kOffB + stage * Cfg::kBBytes;
-                    const uint64_t a_desc = kAMn ? make_smem_desc(sa, 8192, 1024, 2) : make_desc_k_sw128(sa);
-                    const uint64_t b_desc = kBMn ? make_smem_desc(sb, 8192, 1024, 2) : make_desc_k_sw128(sb);
                     if (issuer) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            // descriptor addresses count 16 bytes: a K step is 32 bytes along a K-major row, or 16 K rows
-                            // (2 KB) of an MN-major tile
-                            const uint64_t ad = a_desc + static_cast<uint64_t>(j * (kAMn ? 128 : 2));
-                            const uint64_t bd = b_desc + static_cast<uint64_t>(j * (kBMn ? 128 : 2));
-                            const uint32_t accumulate = (i > 0 || j > 0) ? 1u : 0u;
-                            if constexpr (kInt8) mma_int8<CG>(d_tmem, ad, bd, idesc, accumulate);
-                            else mma_bf16<CG>(d_tmem, ad, bd, idesc, accumulate);
+                        for (int u = 0; u < 2; ++u) {
+                            if (u == kbs) break;
+                            const uint32_t ua = sa + u * a_bytes, ub = sb + u * b_bytes;
+                            const uint64_t a_desc = kAMn ? make_smem_desc(ua, 8192, 1024, 2) : make_desc_k_sw128(ua);
+                            const uint64_t b_desc = kBMn ? make_smem_desc(ub, 8192, 1024, 2) : make_desc_k_sw128(ub);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                // descriptor addresses count 16 bytes: a K step is 32 bytes along a K-major row, or 16 K rows
+                                // (2 KB) of an MN-major tile
+                                const uint64_t ad = a_desc + static_cast<uint64_t>(j * (kAMn ? 128 : 2));
+                                const uint64_t bd = b_desc + static_cast<uint64_t>(j * (kBMn ? 128 : 2));
+                                const uint32_t accumulate = (i > 0 || u > 0 || j > 0) ? 1u : 0u;
+                                if constexpr (kInt8) mma_int8<CG>(d_tmem, ad, bd, idesc, accumulate);
+                                else mma_bf16<CG>(d_tmem, ad, bd, idesc, accumulate);
+                            }
                         }
-                        tcgen05_commit<CG>(bar_empty + stage * 8);
+                        tcgen05_commit<CG>(empty);
                     }
-                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    sa += kbs * a_bytes;
+                    sb += kbs * b_bytes;
+                    full += 8;
+                    empty += 8;
+                    if (full == bar_end) { sa = smem_base; sb = ring_b; full = bar_full; empty = bar_empty; phase ^= 1u; }
                 }
                 if (ok && issuer) tcgen05_commit<CG>(bar_tfull + acc * 8);
                 __syncwarp();
@@ -323,15 +380,15 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     } else {
         // --------------------------------------------------------------- epilogue
         const int quad = warp & 3;             // TMEM lane quadrant this warp may access
-        const int half = (warp - 2) >> 2;      // takes every second group of 64 result columns
-        const uint32_t sbuf = smem_base + Cfg::kOffEpi + (warp - 2) * Cfg::kEpiBufBytes;
-        if (p.pdl) pdl_wait_prior_grid();
+        const int half = (warp - 3) >> 2;      // takes every second group of 64 result columns
+        const uint32_t sbuf = smem_base + Cfg::kOffEpi + (warp - 3) * Cfg::kEpiBufBytes;
+        if (!p.wait_late) pdl_wait_prior_grid();
         const uint32_t tempty0 = (CG == 2) ? mapa_shared(bar_tempty, 0) : bar_tempty;
         const int results = (kGated && p.gate != nullptr) ? 3 : 1;
         int tile_iter = 0;
         for (int t = cluster_id; t < num_tiles; t += num_clusters, ++tile_iter) {
-            int tm, tn;
-            dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn);
+            int tm, tn, split;
+            dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn, split);
             const bool second = tm >= p.tiles_m;
             const int acc = tile_iter & 1;
             const uint32_t acc_phase = static_cast<uint32_t>(tile_iter >> 1) & 1u;
@@ -345,6 +402,36 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
             }
             tcgen05_fence_after();
             const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * 256;
+            if (EPI == kDensePlain && p.splits > 1) {
+                // fp32 sums of a K range: 32 rows x 32 columns at a time through the same transpose
+                float* base = p.partial + (static_cast<long long>(split * p.batches + (second ? 1 : 0)) * p.m) * p.n;
+                for (int c0 = half * 32; c0 < out_cols; c0 += 64) {
+                    uint32_t v[32];
+                    tmem_ld_32x32b_x32(t_acc + c0, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const uint32_t addr = sbuf + lane * 128 + ((q ^ (lane & 7)) << 4);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[4 * q]), "r"(v[4 * q + 1]),
+                                     "r"(v[4 * q + 2]), "r"(v[4 * q + 3])
+                                     : "memory");
+                    }
+                    __syncwarp();
+                    const int q = lane & 7;
+                    const int c = c0 + q * 4;
+                    const bool col_ok = (c < out_cols) && (col0 + c < p.n);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int rr = i * 4 + (lane >> 3);
+                        const uint32_t addr = sbuf + rr * 128 + ((q ^ (rr & 7)) << 4);
+                        uint32_t w0, w1, w2, w3;
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3) : "r"(addr) : "memory");
+                        if (col_ok && row0 + rr < p.m)
+                            *reinterpret_cast<uint4*>(base + static_cast<long long>(row0 + rr) * p.n + col0 + c) = make_uint4(w0, w1, w2, w3);
+                    }
+                    __syncwarp();
+                }
+            } else
             for (int c0 = half * 64; c0 < out_cols; c0 += 128) {
                 for (int r = 0; r < results; ++r) {
                     // 32 rows x 64 columns through a swizzled transpose: lane = row, 16-byte chunk q of a row lives at
@@ -410,10 +497,50 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
         }
     }
 
+    if (p.wait_late) pdl_wait_prior_grid();
     tcgen05_fence_before();
     __syncthreads();
     if constexpr (CG == 2) cluster_sync_all();
     if (warp == 1) tmem_dealloc<CG>(tmem_base, 512);
+}
+
+// Adds up the K ranges of up to three results and rounds once: one thread takes 8 columns of a row.
+struct SplitSum {
+    const float* partial;        // first range; `stride` floats to the next
+    long long stride;
+    __nv_bfloat16* d;
+    long long ldd;
+    long long pieces;            // rows * n / 8
+    int n8;                      // n / 8
+    int splits;
+};
+struct SplitSums {
+    SplitSum job[3];
+};
+
+__global__ void __launch_bounds__(256)
+sum_splits_kernel(const SplitSums p) {
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+#pragma unroll 1
+    for (int j = 0; j < 3; ++j) {
+        const SplitSum& s = p.job[j];
+        for (long long i = blockIdx.x * 256ll + threadIdx.x; i < s.pieces; i += gridDim.x * 256ll) {
+            float acc[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
+            for (int r = 0; r < s.splits; ++r) {
+                const float4* src = reinterpret_cast<const float4*>(s.partial + r * s.stride + i * 8);
+                const float4 lo = __ldcs(src), hi = __ldcs(src + 1);
+                acc[0] += lo.x; acc[1] += lo.y; acc[2] += lo.z; acc[3] += lo.w;
+                acc[4] += hi.x; acc[5] += hi.y; acc[6] += hi.z; acc[7] += hi.w;
+            }
+            const long long row = i / s.n8;
+            const long long col = (i - row * s.n8) * 8;
+            *reinterpret_cast<uint4*>(s.d + row * s.ldd + col) =
+                make_uint4(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]), pack_bf16(acc[4], acc[5]), pack_bf16(acc[6], acc[7]));
+        }
+    }
 }
 
 }  // namespace avefp4

@@ -75,14 +75,12 @@ __device__ __forceinline__ uint2 int8_codes8(const uint4& v, const RowScale& r) 
 template <int NV, bool CTA_ROW>
 __global__ void __launch_bounds__(kInt8Threads)
 quantize_int8_kernel(const __nv_bfloat16* __restrict__ x, long long rows, int k, long long ldx, int8_t* __restrict__ values,
-                     long long ldv, float* __restrict__ scales, int pdl) {
+                     long long ldv, float* __restrict__ scales) {
     constexpr int kRowThreads = CTA_ROW ? kInt8Threads : 32;
     constexpr int kKeep = NV > 0 ? NV : 1;
     __shared__ uint32_t warp_top[kInt8Threads / 32];
-    if (pdl) {
-        pdl_launch_dependents();
-        pdl_wait_prior_grid();
-    }
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row = CTA_ROW ? blockIdx.x : static_cast<long long>(blockIdx.x) * (kInt8Threads / 32) + warp;
     if (!CTA_ROW && row >= rows) return;

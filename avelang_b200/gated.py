@@ -15,17 +15,17 @@ from __future__ import annotations
 
 import torch
 
-from . import _dense, _lib
+from . import _dense
 
 
 def _inputs(x: torch.Tensor, W_gate: torch.Tensor, W_up: torch.Tensor) -> tuple[int, int, int]:
     ldx = _dense.matrix(x, "x", torch.bfloat16)
     m, h = x.shape
-    ldg = _dense.matrix(W_gate, "W_gate", torch.bfloat16, None, x.device)
+    ldg = _dense.matrix(W_gate, "W_gate", torch.bfloat16, None, None, x.device)
     f = W_gate.shape[0]
     if W_gate.shape[1] != h:
         raise ValueError(f"x and W_gate must share H, got {h} and {W_gate.shape[1]}.")
-    ldu = _dense.matrix(W_up, "W_up", torch.bfloat16, (f, h), x.device)
+    ldu = _dense.matrix(W_up, "W_up", torch.bfloat16, f, h, x.device)
     _dense.multiple(f, "F", 8)
     _dense.multiple(h, "H", 8, positive=True)
     return ldx, ldg, ldu
@@ -44,14 +44,14 @@ def gemm_gated_transposed_b(x: torch.Tensor, W_gate: torch.Tensor, W_up: torch.T
     ldx, ldg, ldu = _inputs(x, W_gate, W_up)
     m, h = x.shape
     f = W_gate.shape[0]
-    out = _dense.result(out, "out", (m, f), x.device)
+    out, ldd = _dense.result(out, "out", m, f, x.device)
     gate = up = None
     if save:
-        gate = torch.empty((m, f), dtype=torch.bfloat16, device=x.device)
-        up = torch.empty((m, f), dtype=torch.bfloat16, device=x.device)
+        gate = torch.empty(m, f, dtype=torch.bfloat16, device=x.device)
+        up = torch.empty(m, f, dtype=torch.bfloat16, device=x.device)
     if m and f:
         _dense.call("ave_bf16_gemm_gated", x.device, x.data_ptr(), ldx, W_gate.data_ptr(), ldg, W_up.data_ptr(), ldu, act,
-                    out.data_ptr(), out.stride(0), gate.data_ptr() if save else None, f, up.data_ptr() if save else None, f, m, f, h)
+                    out.data_ptr(), ldd, gate.data_ptr() if save else None, f, up.data_ptr() if save else None, f, m, f, h)
     return (out, gate, up) if save else out
 
 
@@ -70,18 +70,17 @@ def gemm_gated_backward(dout: torch.Tensor, x: torch.Tensor, W_gate: torch.Tenso
     m, h = x.shape
     f = W_gate.shape[0]
     dev = x.device
-    ld = [_dense.matrix(t, name, torch.bfloat16, (m, f), dev) for t, name in ((dout, "dout"), (gate, "gate"), (up, "up"))]
-    dx = torch.empty((m, h), dtype=torch.bfloat16, device=dev) if need_dx else None
-    dw = torch.empty((2, f, h), dtype=torch.bfloat16, device=dev) if need_dw else None
-    dw_gate, dw_up = (dw[0], dw[1]) if need_dw else (None, None)
+    ld = [_dense.matrix(t, name, torch.bfloat16, m, f, dev) for t, name in ((dout, "dout"), (gate, "gate"), (up, "up"))]
+    dx = torch.empty(m, h, dtype=torch.bfloat16, device=dev) if need_dx else None
+    dw = torch.empty(2, f, h, dtype=torch.bfloat16, device=dev) if need_dw else None
+    dw_gate, dw_up = dw.unbind(0) if need_dw else (None, None)
     if not (need_dx or need_dw):
         return dx, dw_gate, dw_up
     if m and f:
-        need = _lib.load().ave_bf16_gated_backward_workspace_bytes(m, f)
-        workspace = torch.empty((need,), dtype=torch.uint8, device=dev)
+        hold, workspace, need = _dense.workspace("ave_bf16_gated_backward", dev, m, f, h, need_dx, need_dw)
         _dense.call("ave_bf16_gated_backward", dev, dout.data_ptr(), ld[0], x.data_ptr(), ldx, W_gate.data_ptr(), ldg, W_up.data_ptr(), ldu,
                     gate.data_ptr(), ld[1], up.data_ptr(), ld[2], act, dx.data_ptr() if need_dx else None, h,
-                    dw_gate.data_ptr() if need_dw else None, dw_up.data_ptr() if need_dw else None, h, workspace.data_ptr(), need, m, f, h)
+                    dw_gate.data_ptr() if need_dw else None, dw_up.data_ptr() if need_dw else None, h, workspace, need, m, f, h)
     else:      # an empty sum
         for d in (dx, dw):
             if d is not None:

@@ -57,25 +57,28 @@ def quantize_int8(x: torch.Tensor, out: Int8Operand | None = None) -> Int8Operan
     rows, k = x.shape
     _dense.multiple(k, "K", 16, positive=True)
     if out is None:
-        out = Int8Operand(torch.empty((rows, k), dtype=torch.int8, device=x.device),
-                          torch.empty((rows,), dtype=torch.float32, device=x.device))
+        out = Int8Operand(torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format),
+                          torch.empty(rows, dtype=torch.float32, device=x.device))
         ldv = k
     else:
-        ldv = _operand(out, "out", x.device, shape=(rows, k))
+        ldv = _operand(out, "out", x.device, rows)
+        if out.k != k:
+            raise ValueError(f"out must have shape {(rows, k)}, got {out.shape}.")
     if rows:
         _dense.call("ave_int8_quantize", x.device, x.data_ptr(), rows, k, ldx, out.values.data_ptr(), ldv, out.scales.data_ptr())
     return out
 
 
-def _operand(op: Int8Operand, name: str, device: torch.device | None = None, k: int | None = None,
-             shape: tuple[int, int] | None = None) -> int:
+def _operand(op: Int8Operand, name: str, device: torch.device | None = None, rows: int | None = None, k: int | None = None) -> int:
     """Check an operand; return its row stride."""
     if not isinstance(op, Int8Operand):
         raise ValueError(f"{name} must be an Int8Operand, got {type(op).__name__}.")
-    ld = _dense.matrix(op.values, f"{name}.values", torch.int8, shape, device)
-    _dense.vector(op.scales, f"{name}.scales", torch.float32, op.values.shape[0], op.values.device)
-    if k is not None and op.values.shape[1] != k:
-        raise ValueError(f"A and {name} must share K, got {k} and {op.values.shape[1]}.")
+    values = op.values
+    ld = _dense.matrix(values, f"{name}.values", torch.int8, rows, None, device)
+    r, c = values.shape
+    if k is not None and c != k:
+        raise ValueError(f"A and {name} must share K, got {k} and {c}.")
+    _dense.vector(op.scales, f"{name}.scales", torch.float32, r, values.device)
     return ld
 
 
@@ -97,16 +100,16 @@ def gemm_int8_transposed_b(A: Int8Operand, B: Int8Operand, out: torch.Tensor | N
     lda = _operand(A, "A")
     m, k = A.values.shape
     dev = A.values.device
-    ldb = _operand(B, "B", dev, k)
+    ldb = _operand(B, "B", dev, None, k)
     n = B.values.shape[0]
     _check_k(k)
     _dense.multiple(n, "N", 8)
     if bias is not None:
         _dense.vector(bias, "bias", torch.bfloat16, n, dev)
-    out = _dense.result(out, "out", (m, n), dev)
+    out, ldd = _dense.result(out, "out", m, n, dev)
     if m and n:
         _dense.call("ave_int8_gemm", dev, A.values.data_ptr(), lda, A.scales.data_ptr(), B.values.data_ptr(), ldb, B.scales.data_ptr(),
-                    None if bias is None else bias.data_ptr(), act, out.data_ptr(), out.stride(0), m, n, k)
+                    None if bias is None else bias.data_ptr(), act, out.data_ptr(), ldd, m, n, k)
     return out
 
 
@@ -120,14 +123,14 @@ def gemm_int8_gated_transposed_b(A: Int8Operand, W_gate: Int8Operand, W_up: Int8
     lda = _operand(A, "A")
     m, k = A.values.shape
     dev = A.values.device
-    ldg = _operand(W_gate, "W_gate", dev, k)
+    ldg = _operand(W_gate, "W_gate", dev, None, k)
     f = W_gate.values.shape[0]
-    ldu = _operand(W_up, "W_up", dev, shape=(f, k))
+    ldu = _operand(W_up, "W_up", dev, f, k)
     _check_k(k)
     _dense.multiple(f, "F", 8)
-    out = _dense.result(out, "out", (m, f), dev)
+    out, ldd = _dense.result(out, "out", m, f, dev)
     if m and f:
         _dense.call("ave_int8_gemm_gated", dev, A.values.data_ptr(), lda, A.scales.data_ptr(), W_gate.values.data_ptr(), ldg,
-                    W_gate.scales.data_ptr(), W_up.values.data_ptr(), ldu, W_up.scales.data_ptr(), act, out.data_ptr(), out.stride(0),
+                    W_gate.scales.data_ptr(), W_up.values.data_ptr(), ldu, W_up.scales.data_ptr(), act, out.data_ptr(), ldd,
                     m, f, k)
     return out

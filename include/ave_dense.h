@@ -55,10 +55,11 @@ int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t 
  * Backward pass of ave_bf16_gemm_gated from dD (m, f) and the kept products gate and up:
  *   dG = dD * up * act'(gate), dU = dD * act(gate)    (rounded to bf16: operands of the products)
  *   dx (m, h) = dG Wg + dU Wu,   dw_gate (f, h) = dG^T X,   dw_up (f, h) = dU^T X.
- * dx, or dw_gate and dw_up together, may be NULL.  `workspace`: ave_bf16_gated_backward_workspace_bytes(m, f) bytes, 256-byte
- * aligned, holds dG and dU during the call; no state is kept in it.  m == 0 writes zeros to dw_gate and dw_up.
+ * dx, or dw_gate and dw_up together, may be NULL.  `workspace`: ave_bf16_gated_backward_workspace_bytes(...) bytes (for the
+ * current device; want_dx / want_dw: whether those results are not NULL), 256-byte aligned; it holds dG and dU, and partial sums
+ * where K is cut into ranges, during the call, and no state between calls.  m == 0 writes zeros to dw_gate and dw_up.
  */
-int64_t ave_bf16_gated_backward_workspace_bytes(int64_t m, int64_t f);
+int64_t ave_bf16_gated_backward_workspace_bytes(int64_t m, int64_t f, int64_t h, int want_dx, int want_dw);
 int ave_bf16_gated_backward(const void* dd, int64_t ld_dd, const void* x, int64_t ldx, const void* w_gate, int64_t ld_wg,
                             const void* w_up, int64_t ld_wu, const void* gate, int64_t ld_gate, const void* up, int64_t ld_up,
                             int activation, void* dx, int64_t ld_dx, void* dw_gate, void* dw_up, int64_t ld_dw, void* workspace,
@@ -66,10 +67,14 @@ int ave_bf16_gated_backward(const void* dd, int64_t ld_dd, const void* x, int64_
 
 /*
  * Gradients of D = A B^T (ave_bf16_gemm): da (m, k) = dD B, db (n, k) = dD^T A, for dD (m, n), A (m, k), B (n, k), read as
- * they lie in memory.  da or db may be NULL.  n % 8 == 0, k % 8 == 0; m == 0 writes zeros to db, n == 0 to da.
+ * they lie in memory.  da or db may be NULL.  n % 8 == 0, k % 8 == 0; m == 0 writes zeros to db, n == 0 to da.  `workspace`:
+ * ave_bf16_gemm_backward_workspace_bytes(...) bytes (for the current device; 0 for most sizes), 256-byte aligned, holds partial
+ * sums during the call.
  */
+int64_t ave_bf16_gemm_backward_workspace_bytes(int64_t m, int64_t n, int64_t k, int want_da, int want_db);
 int ave_bf16_gemm_backward(const void* dd, int64_t ld_dd, const void* a, int64_t lda, const void* b, int64_t ldb, void* da,
-                           int64_t ld_da, void* db, int64_t ld_db, int64_t m, int64_t n, int64_t k, void* stream);
+                           int64_t ld_da, void* db, int64_t ld_db, void* workspace, int64_t workspace_bytes, int64_t m, int64_t n, int64_t k,
+                           void* stream);
 
 #ifdef __cplusplus
 }

@@ -59,18 +59,18 @@ def test_operators_refuse_host_tensors_and_wrong_types():
 def test_matrix_check():
     cpu = torch.device("cpu")
     wide = _bf16(4, 64)
-    assert _dense.matrix(wide, "x", torch.bfloat16, (4, 64), cpu) == 64
-    assert _dense.matrix(wide[:, 8:40], "x", torch.bfloat16, None, cpu) == 64
-    assert _dense.matrix(wide[:1, :24], "x", torch.bfloat16, None, cpu) == 24
-    assert _dense.matrix(wide[:0], "x", torch.bfloat16, None, cpu) == 64
+    assert _dense.matrix(wide, "x", torch.bfloat16, 4, 64, cpu) == 64
+    assert _dense.matrix(wide[:, 8:40], "x", torch.bfloat16, None, None, cpu) == 64
+    assert _dense.matrix(wide[:1, :24], "x", torch.bfloat16, None, None, cpu) == 24
+    assert _dense.matrix(wide[:0], "x", torch.bfloat16, None, None, cpu) == 64
     for bad, match in ((wide[:, 4:36], "16-byte aligned"), (wide.T, "row-major"), (wide[:, ::2], "row-major"), (_bf16(4, 12), "16-byte aligned"),
                        (wide[:1].expand(4, 64), "row-major"), (_bf16(64), "2-D"), (_bf16(2, 4, 8), "2-D"), (wide.float(), "dtype")):
         with pytest.raises(ValueError, match=match):
-            _dense.matrix(bad, "x", torch.bfloat16, None, cpu)
+            _dense.matrix(bad, "x", torch.bfloat16, None, None, cpu)
     with pytest.raises(ValueError, match="must have shape"):
-        _dense.matrix(wide, "x", torch.bfloat16, (4, 72), cpu)
+        _dense.matrix(wide, "x", torch.bfloat16, 4, 72, cpu)
     with pytest.raises(ValueError, match="must be on device"):
-        _dense.matrix(wide, "x", torch.bfloat16, None, torch.device("cuda", 0))
+        _dense.matrix(wide, "x", torch.bfloat16, None, None, torch.device("cuda", 0))
     scales = torch.ones(16)
     _dense.vector(scales[4:12], "s", torch.float32, 8, cpu)
     for bad, match in ((scales[1:9], "16-byte aligned"), (scales[::2], "contiguous"), (scales, "shape"), (scales[:8].double(), "float32")):
@@ -105,19 +105,17 @@ def test_c_entries_refuse_before_any_launch(lib):
     _refused(lib, lib.ave_bf16_gemm_gated(P, 64, P, 64, P, 64, 4, P, 16, P, 16, None, 16, 4, 16, 64, None), "kept together")
     _refused(lib, lib.ave_bf16_gemm_gated(P, 64, P, 64, P, 64, 4, P, 16, None, 16, None, 16, 4, 16, 60, None), "H must be a positive multiple of 8")
     back = lib.ave_bf16_gated_backward
-    need = lib.ave_bf16_gated_backward_workspace_bytes(4, 16)
-    assert need == 512 and lib.ave_bf16_gated_backward_workspace_bytes(-1, 16) < 0
+    assert lib.ave_bf16_gated_backward_workspace_bytes(-1, 16, 64, 1, 1) < 0 and lib.ave_bf16_gemm_backward_workspace_bytes(4, 16, -64, 1, 1) < 0
     ok = [P, 16, P, 64, P, 64, P, 64, P, 16, P, 16, 4, P, 64, P, P, 64]
-    _refused(lib, back(*ok, P, need - 1, 4, 16, 64, None), "the workspace must")
-    _refused(lib, back(*ok, None, need, 4, 16, 64, None), "the workspace must")
-    _refused(lib, back(*ok[:15], P, None, 64, P, need, 4, 16, 64, None), "computed together")
-    _refused(lib, lib.ave_bf16_gemm_backward(P, 16, P, 64, P, 64, P, 60, P, 64, 4, 16, 64, None), "row stride of dA")
-    _refused(lib, lib.ave_bf16_gemm_backward(P, 16, P, 64, P, 64, P, 64, P, 64, 4, 12, 64, None), "N must be a multiple of 8")
+    _refused(lib, back(*ok[:15], P, None, 64, P, 4096, 4, 16, 64, None), "computed together")
+    _refused(lib, back(*ok[:8], P, 12, *ok[10:], P, 4096, 4, 16, 64, None), "row stride of gate")
+    _refused(lib, lib.ave_bf16_gemm_backward(P, 16, P, 64, P, 64, P, 60, P, 64, None, 0, 4, 16, 64, None), "row stride of dA")
+    _refused(lib, lib.ave_bf16_gemm_backward(P, 16, P, 64, P, 64, P, 64, P, 64, None, 0, 4, 12, 64, None), "N must be a multiple of 8")
 
 
 def test_calls_before_init_fail_loudly(lib):
     if torch.cuda.is_available():
         pytest.skip("a GPU is present; this checks the no-device path")
     assert lib.ave_int8_quantize(P, 4, 32, 32, P, 32, P, None) != 0
-    assert lib.ave_bf16_gemm_backward(P, 16, P, 64, P, 64, P, 64, P, 64, 4, 16, 64, None) != 0
+    assert lib.ave_bf16_gemm_backward(P, 16, P, 64, P, 64, P, 64, P, 64, None, 0, 4, 16, 64, None) != 0
     assert lib.ave_fp4_last_error()
