@@ -138,37 +138,47 @@ __device__ __forceinline__ void dense_tile(int t, int rows, int cols, int band, 
     tn = r / in_band;
 }
 
-// 32 accumulator columns of this thread's row -> 16 words of bf16 pairs.  `col` is the first one's column in the result.
-template <bool INT8, int EPI, int ACT>
-__device__ __forceinline__ void dense_convert(const uint32_t (&v)[32], const uint32_t (&u)[32], uint32_t (&w)[16], float sa,
-                                              const float* sb0, const float* sb1, const __nv_bfloat16* bias, int col, int n) {
+// 16 accumulator columns of this thread's row -> 8 words of bf16 pairs.  `col` is the first one's column in the result.
+// (16 and not more at a time keeps the code of five activations small: a short launch runs it from a cold instruction cache.)
+template <bool INT8, int EPI>
+struct ColumnTerms {
+    float4 s0[INT8 ? 4 : 1], s1[INT8 && EPI == kDenseGated ? 4 : 1];
+    uint2 bias[EPI == kDenseScaled ? 4 : 1];
+};
+
+// Scales and bias of 16 columns from `col` on; the ones past the last column stand in for any.  n is a multiple of 8.
+template <bool INT8, int EPI>
+__device__ __forceinline__ void load_terms(ColumnTerms<INT8, EPI>& t, const float* sb0, const float* sb1, const __nv_bfloat16* bias, int col, int n) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        float4 s0 = make_float4(1.0f, 1.0f, 1.0f, 1.0f), s1 = s0;
-        float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (col + 4 * q < n) {          // n is a multiple of 8
-            if constexpr (INT8) {
-                s0 = __ldg(reinterpret_cast<const float4*>(sb0 + col) + q);
-                if constexpr (EPI == kDenseGated) s1 = __ldg(reinterpret_cast<const float4*>(sb1 + col) + q);
-            }
-            if constexpr (EPI == kDenseScaled) {
-                if (bias != nullptr) {
-                    const uint2 bw = __ldg(reinterpret_cast<const uint2*>(bias + col) + q);
-                    b[0] = bf16_lo(bw.x); b[1] = bf16_hi(bw.x); b[2] = bf16_lo(bw.y); b[3] = bf16_hi(bw.y);
-                }
-            }
+    for (int q = 0; q < 4; ++q) {
+        const int at = min(col + 4 * q, n - 4);
+        if constexpr (INT8) {
+            t.s0[q] = __ldg(reinterpret_cast<const float4*>(sb0 + at));
+            if constexpr (EPI == kDenseGated) t.s1[q] = __ldg(reinterpret_cast<const float4*>(sb1 + at));
         }
-        const float c0[4] = {s0.x, s0.y, s0.z, s0.w}, c1[4] = {s1.x, s1.y, s1.z, s1.w};
-        float y[4];
+        if constexpr (EPI == kDenseScaled) t.bias[q] = (bias != nullptr) ? __ldg(reinterpret_cast<const uint2*>(bias + at)) : make_uint2(0u, 0u);
+    }
+}
+
+template <bool INT8, int EPI, int ACT>
+__device__ __forceinline__ void dense_convert(const uint32_t (&v)[16], const uint32_t (&u)[16], uint32_t (&w)[8], float sa,
+                                              const ColumnTerms<INT8, EPI>& t) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float c0[4], c1[4], b[4], y[4];
+        if constexpr (INT8) { c0[0] = t.s0[q].x; c0[1] = t.s0[q].y; c0[2] = t.s0[q].z; c0[3] = t.s0[q].w; }
+        if constexpr (INT8 && EPI == kDenseGated) { c1[0] = t.s1[q].x; c1[1] = t.s1[q].y; c1[2] = t.s1[q].z; c1[3] = t.s1[q].w; }
+        if constexpr (EPI == kDenseScaled) { b[0] = bf16_lo(t.bias[q].x); b[1] = bf16_hi(t.bias[q].x); b[2] = bf16_lo(t.bias[q].y); b[3] = bf16_hi(t.bias[q].y); }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             // int32 -> fp32 rounds to nearest: 2^-24 of the sum, far below the one rounding to bf16.  The channel's scale comes
             // first: weights are of ordinary size, so the product with a large token's scale overflows only if the result does.
-            float g = INT8 ? __int2float_rn(static_cast<int>(v[4 * q + i])) * c0[i] * sa : __uint_as_float(v[4 * q + i]);
+            float g = __uint_as_float(v[4 * q + i]);
+            if constexpr (INT8) g = __int2float_rn(static_cast<int>(v[4 * q + i])) * c0[i] * sa;
             if constexpr (EPI == kDenseScaled) g += b[i];
             y[i] = act_value<ACT>(g);
-            if constexpr (EPI == kDenseGated)
-                y[i] *= INT8 ? __int2float_rn(static_cast<int>(u[4 * q + i])) * c1[i] * sa : __uint_as_float(u[4 * q + i]);
+            if constexpr (EPI == kDenseGated && INT8) y[i] *= __int2float_rn(static_cast<int>(u[4 * q + i])) * c1[i] * sa;
+            if constexpr (EPI == kDenseGated && !INT8) y[i] *= __uint_as_float(u[4 * q + i]);
         }
         w[2 * q] = pack_bf16(y[0], y[1]);
         w[2 * q + 1] = pack_bf16(y[2], y[3]);
@@ -380,7 +390,8 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     } else {
         // --------------------------------------------------------------- epilogue
         const int quad = warp & 3;             // TMEM lane quadrant this warp may access
-        const int half = (warp - 3) >> 2;      // takes every second group of 64 result columns
+        const int half = (warp - 3) >> 2;      // takes every second group of `unit` result columns
+        const int unit = (out_cols > 64) ? 64 : 32;
         const uint32_t sbuf = smem_base + Cfg::kOffEpi + (warp - 3) * Cfg::kEpiBufBytes;
         if (!p.wait_late) pdl_wait_prior_grid();
         const uint32_t tempty0 = (CG == 2) ? mapa_shared(bar_tempty, 0) : bar_tempty;
@@ -395,7 +406,10 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
             const int row0 = ((second ? tm - p.tiles_m : tm) * CG + rank) * 128 + quad * 32;
             const int col0 = tn * out_cols;
             float sa = 1.0f;
+            // the row's scale and the first columns' scales and bias come while the products still run
             if constexpr (kInt8) sa = (row0 + lane < p.m) ? __ldg(p.a_scale + row0 + lane) : 0.0f;
+            ColumnTerms<kInt8, EPI> terms;
+            load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col0 + half * unit, p.n);
             if (!mbar_wait(bar_tfull + acc * 8, acc_phase)) {
                 if (lane == 0) atomicCAS(p.status, 0, 103);
                 break;
@@ -432,37 +446,36 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
                     __syncwarp();
                 }
             } else
-            for (int c0 = half * 64; c0 < out_cols; c0 += 128) {
+            for (int c0 = half * unit; c0 < out_cols; c0 += 2 * unit) {
+                const int c1 = min(c0 + unit, out_cols);
                 for (int r = 0; r < results; ++r) {
-                    // 32 rows x 64 columns through a swizzled transpose: lane = row, 16-byte chunk q of a row lives at
-                    // chunk q ^ (row & 7); every store below then writes whole 128-byte lines
+                    // 32 rows x up to 64 columns through a swizzled transpose: lane = row, 16-byte chunk q of a row lives at
+                    // chunk q ^ (row & 7); a row's part of the result is then stored by neighbouring lanes
 #pragma unroll 1
-                    for (int h = 0; h < 2; ++h) {
-                        const int c = c0 + h * 32;
-                        if (c >= out_cols) break;
-                        uint32_t v[32], u[32], w[16];
-                        if (!kGated || r < 2) tmem_ld_32x32b_x32(t_acc + c, v);
-                        if constexpr (kGated) {
-                            if (r == 0) tmem_ld_32x32b_x32(t_acc + out_cols + c, u);
-                            if (r == 2) tmem_ld_32x32b_x32(t_acc + out_cols + c, v);
-                        }
+                    for (int c = c0; c < c1; c += 16) {
+                        uint32_t v[16], u[16], w[8];
+                        tmem_ld_32x32b_x16(t_acc + c + ((kGated && r == 2) ? out_cols : 0), v);
+                        if (kGated && r == 0) tmem_ld_32x32b_x16(t_acc + out_cols + c, u);
                         tmem_ld_wait();
-                        if (kGated && r > 0) {
-                            dense_convert<false, kDensePlain, AVE_FP4_ACT_NONE>(v, v, w, sa, nullptr, nullptr, nullptr, col0 + c, p.n);
-                        } else if constexpr (EPI == kDensePlain) {
-                            dense_convert<false, kDensePlain, AVE_FP4_ACT_NONE>(v, v, w, sa, nullptr, nullptr, nullptr, col0 + c, p.n);
+                        if (EPI == kDensePlain || r > 0) {
+                            dense_convert<false, kDensePlain, AVE_FP4_ACT_NONE>(v, v, w, sa, ColumnTerms<false, kDensePlain>{});
                         } else {
                             switch (p.act) {   // warp-uniform
-                                case AVE_FP4_ACT_RELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_RELU>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
-                                case AVE_FP4_ACT_GELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
-                                case AVE_FP4_ACT_GELU_TANH: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU_TANH>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
-                                case AVE_FP4_ACT_SILU: dense_convert<kInt8, EPI, AVE_FP4_ACT_SILU>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
-                                default: dense_convert<kInt8, EPI, AVE_FP4_ACT_NONE>(v, u, w, sa, p.b_scale[0], p.b_scale[1], p.bias, col0 + c, p.n); break;
+                                case AVE_FP4_ACT_RELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_RELU>(v, u, w, sa, terms); break;
+                                case AVE_FP4_ACT_GELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU>(v, u, w, sa, terms); break;
+                                case AVE_FP4_ACT_GELU_TANH: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU_TANH>(v, u, w, sa, terms); break;
+                                case AVE_FP4_ACT_SILU: dense_convert<kInt8, EPI, AVE_FP4_ACT_SILU>(v, u, w, sa, terms); break;
+                                default: dense_convert<kInt8, EPI, AVE_FP4_ACT_NONE>(v, u, w, sa, terms); break;
                             }
                         }
+                        if constexpr (kInt8) {      // the next 16 columns' terms: in this group, or the first of the next one
+                            const int next = (c + 16 < c1) ? c + 16 : c0 + 2 * unit;
+                            load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col0 + next, p.n);
+                        }
+                        const int q0 = (c - c0) / 8;
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const uint32_t addr = sbuf + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4);
+                        for (int q = 0; q < 2; ++q) {
+                            const uint32_t addr = sbuf + lane * 128 + (((q0 + q) ^ (lane & 7)) << 4);
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[4 * q]), "r"(w[4 * q + 1]),
                                          "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
                                          : "memory");
@@ -475,7 +488,7 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
                     if (kGated && r == 2) { d = p.up; ld = p.ld_up; }
                     const int q = lane & 7;
                     const int c = c0 + q * 8;
-                    const bool col_ok = (c < out_cols) && (col0 + c < p.n);
+                    const bool col_ok = (c < c1) && (col0 + c < p.n);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int rr = i * 4 + (lane >> 3);
