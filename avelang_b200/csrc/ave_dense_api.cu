@@ -346,6 +346,25 @@ cudaError_t prepare_dense_kernels() {
     PREP(false, true, true)
     PREP(false, true, false)
 #undef PREP
+    // the others are only looked at, so that their code is on the device before a first call inside a stream capture
+    cudaFuncAttributes attr;
+#define PREP(...) \
+    if ((e = cudaFuncGetAttributes(&attr, __VA_ARGS__)) != cudaSuccess) return e;
+    PREP(quantize_int8_kernel<1, false>)
+    PREP(quantize_int8_kernel<2, false>)
+    PREP(quantize_int8_kernel<4, false>)
+    PREP(quantize_int8_kernel<1, true>)
+    PREP(quantize_int8_kernel<2, true>)
+    PREP(quantize_int8_kernel<4, true>)
+    PREP(quantize_int8_kernel<8, true>)
+    PREP(quantize_int8_kernel<0, true>)
+    PREP(gated_backward_kernel<AVE_FP4_ACT_NONE>)
+    PREP(gated_backward_kernel<AVE_FP4_ACT_RELU>)
+    PREP(gated_backward_kernel<AVE_FP4_ACT_GELU>)
+    PREP(gated_backward_kernel<AVE_FP4_ACT_GELU_TANH>)
+    PREP(gated_backward_kernel<AVE_FP4_ACT_SILU>)
+    PREP(sum_splits_kernel)
+#undef PREP
     return cudaSuccess;
 }
 

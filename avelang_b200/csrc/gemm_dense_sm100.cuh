@@ -248,14 +248,16 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     tcgen05_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_gen, 0);
 
+    // Operands may come from the previous kernel.  All roles wait for it here, so that none of the bounded waits below counts its time.
+    if (threadIdx.x == 0 && !p.trigger_late) pdl_launch_dependents();
+    if (!p.wait_late) pdl_wait_prior_grid();
+    if (threadIdx.x == 0 && p.trigger_late) pdl_launch_dependents();
+
     if (warp == 0 || warp == 2) {
         // ------------------------------------------------------- TMA producers: warp 0 loads A, warp 2 loads B
         // Each walks the whole schedule; with one warp for both, the issue loop and not the copies set the pace of narrow tiles.
         const bool for_a = (warp == 0);
         const bool issuer = elect_one_sync();
-        if (issuer && !p.trigger_late) pdl_launch_dependents();
-        if (!p.wait_late) pdl_wait_prior_grid();       // operands may come from the previous kernel
-        if (issuer && p.trigger_late) pdl_launch_dependents();
         // operands that other CTAs read as well stay in L2; with a single tile row B passes through once
         const uint64_t policy = (!for_a && tile_rows == 1) ? kL2EvictFirst : kL2EvictLast;
         const uint32_t bytes = static_cast<uint32_t>(for_a ? a_bytes : b_bytes);
@@ -393,7 +395,6 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
         const int half = (warp - 3) >> 2;      // takes every second group of `unit` result columns
         const int unit = (out_cols > 64) ? 64 : 32;
         const uint32_t sbuf = smem_base + Cfg::kOffEpi + (warp - 3) * Cfg::kEpiBufBytes;
-        if (!p.wait_late) pdl_wait_prior_grid();
         const uint32_t tempty0 = (CG == 2) ? mapa_shared(bar_tempty, 0) : bar_tempty;
         const int results = (kGated && p.gate != nullptr) ? 3 : 1;
         int tile_iter = 0;

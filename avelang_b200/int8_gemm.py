@@ -74,11 +74,11 @@ def _operand(op: Int8Operand, name: str, device: torch.device | None = None, row
     if not isinstance(op, Int8Operand):
         raise ValueError(f"{name} must be an Int8Operand, got {type(op).__name__}.")
     values = op.values
-    ld = _dense.matrix(values, f"{name}.values", torch.int8, rows, None, device)
+    ld = _dense.matrix(values, name + ".values", torch.int8, rows, None, device)
     r, c = values.shape
     if k is not None and c != k:
         raise ValueError(f"A and {name} must share K, got {k} and {c}.")
-    _dense.vector(op.scales, f"{name}.scales", torch.float32, r, values.device)
+    _dense.vector(op.scales, name + ".scales", torch.float32, r, device or values.device)
     return ld
 
 

@@ -119,3 +119,19 @@ def test_calls_before_init_fail_loudly(lib):
     assert lib.ave_int8_quantize(P, 4, 32, 32, P, 32, P, None) != 0
     assert lib.ave_bf16_gemm_backward(P, 16, P, 64, P, 64, P, 64, P, 64, None, 0, 4, 16, 64, None) != 0
     assert lib.ave_fp4_last_error()
+
+
+def test_operators_are_importable_under_the_reference_package_name():
+    import importlib
+    import sys
+
+    sys.path.insert(0, os.path.join(ROOT, "python"))
+    try:
+        i8 = importlib.import_module("avelang_kernels.int8_gemm")
+        gated = importlib.import_module("avelang_kernels.gated")
+    finally:
+        sys.path.remove(os.path.join(ROOT, "python"))
+    for name in i8.__all__:
+        assert getattr(i8, name) is getattr(ave.int8_gemm, name)
+    for name in gated.__all__:
+        assert getattr(gated, name) is getattr(ave, name)

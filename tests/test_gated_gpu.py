@@ -213,3 +213,96 @@ def test_training_step_on_a_side_stream_and_in_a_graph(cuda_device):
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(captured, step()))
     ave.check_device_status(cuda_device)
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 8200, 64), (8200, 40, 64), (9, 4096, 16), (300, 16392, 72), (8200, 264, 136), (130, 5000, 200)])
+def test_long_sums_of_few_tiles(cuda_device, m, n, k):
+    """Products of a few tiles and long sums: K is cut into ranges whose sums are added by a kernel of their own."""
+    a, b, dout = _randn(cuda_device, m, k, 1), _randn(cuda_device, n, k, 2, k ** -0.5), _randn(cuda_device, m, n, 3, 0.1)
+    got = ave.gemm_transposed_b_backward(dout, a, b)
+    for g, w, what in zip(got, D.product_backward(dout, a, b), ("da", "db")):
+        D.check(g, w, what)
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(got, ave.gemm_transposed_b_backward(dout, a, b)))
+    f, h = n, k
+    wg, wu = _randn(cuda_device, f, h, 5, h ** -0.5), _randn(cuda_device, f, h, 6, h ** -0.5)
+    gate, up = _randn(cuda_device, m, f, 7), _randn(cuda_device, m, f, 8)
+    for g, w, what in zip(ave.gemm_gated_backward(dout, a, wg, wu, gate, up), D.gated_backward(dout, a, wg, wu, gate, up, "silu"), ("dx", "dw_gate", "dw_up")):
+        D.check(g, w, what)
+    ave.check_device_status(cuda_device)
+
+
+def test_kept_products_feed_the_backward_pass_for_few_rows(cuda_device):
+    """save=True on the streaming kernel (up to 16 rows) and on either side of its rule for large weights."""
+    for m, f, h in ((1, 520, 264), (8, 8200, 1032), (9, 8200, 1032), (16, 4104, 2056), (12, 16, 8)):
+        x, wg, wu = _block(cuda_device, m, f, h)
+        kept = ave.gemm_gated_transposed_b(x, wg, wu, activation="gelu", save=True)
+        for got, w, what in zip(kept, D.gated(x, wg, wu, "gelu"), ("out", "gate", "up")):
+            D.check(got, w, f"{m}x{f}x{h} {what}")
+        dout = _randn(cuda_device, m, f, 4, 0.1)
+        for g, w in zip(ave.gemm_gated_backward(dout, x, wg, wu, *kept[1:], activation="gelu"),
+                        D.gated_backward(dout, x, wg, wu, *kept[1:], "gelu")):
+            D.check(g, w, f"{m}x{f}x{h}")
+    ave.check_device_status(cuda_device)
+
+
+def test_backward_captured_twice_and_replayed_at_once(cuda_device):
+    """Two captured backward passes on streams of their own at the same time, next to eager calls: each has its own workspace."""
+    m, f, h = 150, 1032, 264
+    x, wg, wu = _block(cuda_device, m, f, h)
+    gate, up = _randn(cuda_device, m, f, 5), _randn(cuda_device, m, f, 6)
+    douts = [_randn(cuda_device, m, f, s, 0.1) for s in (7, 8, 9)]
+    want = [ave.gemm_gated_backward(d, x, wg, wu, gate, up) for d in douts]
+    graphs, got = [], []
+    for d in douts[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(ave.gemm_gated_backward(d, x, wg, wu, gate, up))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(3)]
+    torch.cuda.synchronize()
+    eager = []
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        with torch.cuda.stream(streams[2]):
+            eager.append(ave.gemm_gated_backward(douts[2], x, wg, wu, gate, up))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(p, q) for p, q in zip(got[i], want[i]))
+    for e in eager:
+        assert all(torch.equal(p, q) for p, q in zip(e, want[2]))
+    ave.check_device_status(cuda_device)
+
+
+def test_first_call_of_each_operator_inside_a_capture(cuda_device):
+    """A fresh process: after the library's set-up, every operator's first call ever is a captured one."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch, avelang_b200 as ave
+from avelang_b200 import _lib
+_lib.ensure_init(0)
+bf = torch.bfloat16
+x, w = torch.randn(40, 64, device="cuda").to(bf), torch.randn(72, 64, device="cuda").to(bf)
+def everything():
+    q, v = ave.quantize_int8(x), ave.quantize_int8(w)
+    out, gate, up = ave.gemm_gated_transposed_b(x, w, w, save=True)
+    return (q.values, ave.gemm_int8_transposed_b(q, v), ave.gemm_int8_gated_transposed_b(q, v, v), out, gate, up,
+            *ave.gemm_gated_backward(out, x, w, w, gate, up), *ave.gemm_transposed_b_backward(out, x, w))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = everything()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, everything()))
+ave.check_device_status()
+print("fine")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "fine" in run.stdout, run.stdout + run.stderr

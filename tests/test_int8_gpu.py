@@ -212,3 +212,58 @@ def test_serving_block_on_a_side_stream_and_in_graphs(cuda_device, m):
         want = block(inputs[i])
         assert torch.equal(results[i][1], want[1])
     ave.check_device_status(cuda_device)
+
+
+def test_nine_to_sixteen_rows_on_large_weights(cuda_device):
+    """More than 32 MB of weights go to the tile kernel from 9 rows on, less to the streaming kernel: both sides of the rule."""
+    for n, k in ((8456, 4112), (7912, 4112)):
+        b = _ints(cuda_device, n, k, 2)
+        for m in (8, 9, 16):
+            a = _ints(cuda_device, m, k, m)
+            D.check(ave.gemm_int8_transposed_b(a, b, activation="silu"), D.int8_gemm(a, b, None, "silu"), f"{m}x{n}x{k}")
+    wg, wu = _ints(cuda_device, 4264, 4112, 5), _ints(cuda_device, 4264, 4112, 6)
+    for m in (9, 13, 16):
+        a = _ints(cuda_device, m, 4112, m)
+        D.check(ave.gemm_int8_gated_transposed_b(a, wg, wu), D.int8_gated(a, wg, wu, "silu"), f"gated {m}")
+    ave.check_device_status(cuda_device)
+
+
+def test_results_beyond_two_to_the_31_elements(cuda_device):
+    m, n, k = 66000, 32776, 32
+    a, b = _ints(cuda_device, m, k, 1), _ints(cuda_device, n, k, 2)
+    got = ave.gemm_int8_transposed_b(a, b)
+    for rows in (slice(0, 3), slice(32767, 32771), slice(65530, 65540), slice(m - 3, m)):
+        part = ave.Int8Operand(a.values[rows], a.scales[rows].clone())
+        D.check(got[rows], D.int8_gemm(part, b), f"{rows}")
+    x = got[:, :16384]      # 1.08e9 elements at a row stride of 32776
+    q = ave.quantize_int8(x)
+    for rows in (slice(0, 2), slice(65533, 65540), slice(m - 2, m)):
+        values, scales = D.quantize_int8(x[rows])
+        assert torch.equal(q.values[rows], values) and torch.equal(q.scales[rows], scales.float())
+    ave.check_device_status(cuda_device)
+
+
+def test_two_host_threads_on_streams_of_their_own(cuda_device):
+    import threading
+
+    shapes = [(1, 1000, 1024), (40, 520, 272), (300, 264, 528), (16, 4104, 1040)]
+    cases = [(_ints(cuda_device, m, k, 1), _ints(cuda_device, n, k, 2)) for m, n, k in shapes]
+    want = [ave.gemm_int8_transposed_b(a, b, activation="gelu") for a, b in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(seed):
+        stream = torch.cuda.Stream(cuda_device)
+        with torch.cuda.stream(stream):
+            for i in range(100):
+                j = (i * seed) % len(cases)
+                if not torch.equal(ave.gemm_int8_transposed_b(*cases[j], activation="gelu"), want[j]):
+                    bad.append((seed, i))
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in (1, 3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    ave.check_device_status(cuda_device)
