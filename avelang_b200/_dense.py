@@ -69,6 +69,14 @@ def multiple(value: int, name: str, of: int, positive: bool = False) -> None:
 
 
 _functions: dict = {}
+MIN_CUT_BYTES = 4096      # AVE_DENSE_MIN_CUT_BYTES of include/ave_dense.h: shorter rows of K never need a workspace
+
+
+def forward_workspace(name: str, device: torch.device, m: int, n: int, k: int, k_bytes: int) -> tuple[torch.Tensor | None, int, int]:
+    """Workspace of a forward product; few rows and short K are known to need none."""
+    if k_bytes < MIN_CUT_BYTES or m <= 8:
+        return None, 0, 0
+    return workspace(name, device, m, n, k)
 
 
 def _function(name: str, dev: int):

@@ -34,7 +34,8 @@ EXPORTS = (
 
 # every symbol include/ave_dense.h declares
 DENSE_EXPORTS = (
-    "ave_int8_quantize", "ave_int8_gemm", "ave_int8_gemm_gated", "ave_bf16_gemm_gated", "ave_bf16_gated_backward",
+    "ave_int8_quantize", "ave_int8_gemm", "ave_int8_gemm_workspace_bytes", "ave_int8_gemm_gated", "ave_int8_gemm_gated_workspace_bytes",
+    "ave_bf16_gemm_gated", "ave_bf16_gemm_gated_workspace_bytes", "ave_bf16_gated_backward",
     "ave_bf16_gated_backward_workspace_bytes", "ave_bf16_gemm_backward", "ave_bf16_gemm_backward_workspace_bytes",
 )
 
@@ -102,11 +103,15 @@ def load() -> ctypes.CDLL:
         L.ave_int8_quantize.restype = i32
         L.ave_int8_quantize.argtypes = [vp, i64, i64, i64, vp, i64, vp, vp]
         L.ave_int8_gemm.restype = i32
-        L.ave_int8_gemm.argtypes = [vp, i64, vp, vp, i64, vp, vp, i32, vp, i64, i64, i64, i64, vp]
+        L.ave_int8_gemm.argtypes = [vp, i64, vp, vp, i64, vp, vp, i32, vp, i64, vp, i64, i64, i64, i64, vp]
         L.ave_int8_gemm_gated.restype = i32
-        L.ave_int8_gemm_gated.argtypes = [vp, i64, vp, vp, i64, vp, vp, i64, vp, i32, vp, i64, i64, i64, i64, vp]
+        L.ave_int8_gemm_gated.argtypes = [vp, i64, vp, vp, i64, vp, vp, i64, vp, i32, vp, i64, vp, i64, i64, i64, i64, vp]
         L.ave_bf16_gemm_gated.restype = i32
-        L.ave_bf16_gemm_gated.argtypes = [vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i64, vp, i64, i64, i64, i64, vp]
+        L.ave_bf16_gemm_gated.argtypes = [vp, i64, vp, i64, vp, i64, i32, vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, i64, vp]
+        for name in ("ave_int8_gemm", "ave_int8_gemm_gated", "ave_bf16_gemm_gated"):
+            query = getattr(L, name + "_workspace_bytes")
+            query.restype = i64
+            query.argtypes = [i64, i64, i64]
         L.ave_bf16_gated_backward_workspace_bytes.restype = i64
         L.ave_bf16_gated_backward_workspace_bytes.argtypes = [i64, i64, i64, i32, i32]
         L.ave_bf16_gated_backward.restype = i32

@@ -54,6 +54,12 @@ int check_vector(const char* fn, const char* name, const void* p) {
     return 0;
 }
 
+int check_workspace(const char* fn, const void* workspace, int64_t have, int64_t need) {
+    if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || have < need))
+        return fail("%s: the workspace must be 256-byte aligned and hold %lld bytes", fn, static_cast<long long>(need));
+    return 0;
+}
+
 int check_activation(const char* fn, int act) {
     if (act < AVE_FP4_ACT_NONE || act > AVE_FP4_ACT_SILU) return fail("%s: unknown activation %d", fn, act);
     return 0;
@@ -150,6 +156,9 @@ DensePlan plan_dense(int sms, int64_t m, int64_t cols, int64_t k_bytes, int segm
 template <int OP>
 constexpr int64_t elem_bytes() { return OP == kOpInt8 ? 1 : 2; }
 
+// Forward products cut K only from here on: below they ask for no workspace, and a caller need not ask.
+bool forward_may_cut(int64_t m, int64_t k_bytes) { return m > 8 && k_bytes >= AVE_DENSE_MIN_CUT_BYTES; }
+
 // m, n: sizes of one result; k: sum length of one segment.  A plan depends on the sizes alone and takes a few microseconds
 // to find, as long as a small product runs: each host thread keeps the last ones it made.
 template <int OP, int EPI>
@@ -165,7 +174,7 @@ DensePlan plan_for(const HostDevice& dev, int64_t m, int64_t n, int64_t k, int s
     Slot& slot = slots[((h * 0xD6E8FEB86659FD93ull) >> 32) % kSlots];
     if (slot.m != m || slot.n != n || slot.k != k || slot.sms != dev.sm_count || slot.segments != segments || slot.batches != batches) {
         slot.plan = plan_dense(dev.sm_count, m, EPI == kDenseGated ? 2 * n : n, k * elem_bytes<OP>(), segments, batches, OP == kOpBf16Tn,
-                               OP == kOpBf16Nn || OP == kOpBf16Tn, EPI == kDenseGated, EPI == kDensePlain);
+                               OP == kOpBf16Nn || OP == kOpBf16Tn, EPI == kDenseGated, EPI == kDensePlain || forward_may_cut(m, k * elem_bytes<OP>()));
         slot.m = m;
         slot.n = n;
         slot.k = k;
@@ -211,7 +220,10 @@ int launch_dense_cg(const HostDevice& dev, const DensePlan& plan, const Operand 
     }
     const int64_t items = int64_t(p.tiles_m) * p.batches * p.tiles_n * p.splits;
     const int64_t clusters = dev.sm_count / CG;
-    Launch launch((items < clusters ? items : clusters) * CG, Cfg::kThreads, Cfg::kSmemBytes, CG, stream);
+    // 16 epilogue warps hide more latency (int8 8192 x 8192 x 1024 78 -> 63 us), 8 start sooner (64 x 64 x 64 3.6 against 4.0 us):
+    // tiles of up to 64 result columns keep two warps of a quadrant busy and no more, and the plain epilogue is short.
+    const int threads = Cfg::threads(EPI != kDensePlain && out_cols > 64 ? 16 : 8);
+    Launch launch((items < clusters ? items : clusters) * CG, threads, Cfg::kSmemBytes, CG, stream);
     AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, gemm_dense_kernel<CG, OP, EPI>, ta[0], ta[1], tb[0], tb[1], p));
     return 0;
 }
@@ -224,9 +236,9 @@ int launch_dense(const HostDevice& dev, const DensePlan& plan, const Operand (&a
     return launch_dense_cg<2, OP, EPI>(dev, plan, a, b, m, n, k, p, stream);
 }
 
-int64_t split_floats(const DensePlan& plan, int64_t rows, int64_t n) { return plan.splits > 1 ? plan.splits * rows * n : 0; }
+int64_t split_words(const DensePlan& plan, int64_t rows, int64_t n) { return plan.splits > 1 ? plan.splits * rows * n : 0; }
 
-SplitSum split_sum(const DensePlan& plan, const float* partial, int64_t stride, void* d, int64_t ldd, int64_t rows, int64_t n) {
+SplitSum split_sum(const DensePlan& plan, const uint32_t* partial, int64_t stride, void* d, int64_t ldd, int64_t rows, int64_t n) {
     return SplitSum{partial, stride, static_cast<__nv_bfloat16*>(d), ldd, plan.splits > 1 ? rows * n / 8 : 0, static_cast<int>(n / 8), plan.splits};
 }
 
@@ -241,6 +253,49 @@ int launch_sums(const HostDevice& dev, const SplitSums& sums, cudaStream_t strea
     return 0;
 }
 
+// The streaming kernel works in units of 16 weight rows, of about a microsecond each however short K is, and takes K in steps of
+// 4 KB; the tile kernel needs a long K to fill its pipeline, and does without either.  us, streaming / tile: int8 1 x 1600 x 8192
+// 5.7 / 11.6, 1 x 4800 x 8192 11.3 / 12.4, 1 x 9600 x 8192 17.7 / 17.3, 1 x 28672 x 4096 24.2 / 23.1, 6 x 28672 x 6144 37.6 / 32.2,
+// 1 x 28672 x 8192 39.2 / 42.3, gated 1 x 28672 x 8192 72 / 77.  For 9 to 16 rows its activations do not fit L1 beside the
+// ring: 16 x 1024 x 8192 6.1 / 13.3, 16 x 4096 x 4096 8.0 / 7.7, 16 x 28672 x 8192 48.6 / 42.5.
+bool stream_rows(const HostDevice& dev, int64_t m, int64_t weight_rows, int64_t k_bytes) {
+    const int64_t units = (weight_rows + 15) / 16;
+    if (m <= 8) return units <= 2 * dev.sm_count || (k_bytes >= 8192 && k_bytes % 4096 == 0);
+    return m <= 16 && units <= dev.sm_count;
+}
+
+// A scaled or gated product, with its sums over K cut into ranges where the plan says so.
+template <int OP, int EPI>
+int launch_forward(const HostDevice& dev, const char* fn, const Operand (&a)[2], const Operand (&b)[2], int64_t m, int64_t n, int64_t k,
+                   DenseParams p, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+    const DensePlan plan = plan_for<OP, EPI>(dev, m, n, k, 1, 1);
+    int rc = check_workspace(fn, workspace, workspace_bytes, 4 * split_words(plan, m, EPI == kDenseGated ? 2 * n : n));
+    if (rc) return rc;
+    p.partial = static_cast<uint32_t*>(workspace);
+    rc = launch_dense<OP, EPI>(dev, plan, a, b, m, n, k, p, stream);
+    if (rc || plan.splits == 1) return rc;
+    p.m = static_cast<int>(m);
+    p.n = static_cast<int>(n);
+    p.splits = plan.splits;
+    int64_t grid = ceil_div(m * (n / 8), 256);
+    if (grid > int64_t(dev.sm_count) * 8) grid = int64_t(dev.sm_count) * 8;
+    Launch launch(grid, 256, 0, 1, stream);
+    AVE_CUDA(cudaLaunchKernelEx(&launch.cfg, finish_splits_kernel<OP == kOpInt8, EPI>, p));
+    return 0;
+}
+
+template <int OP, int EPI>
+int64_t forward_workspace(const char* fn, int64_t m, int64_t n, int64_t k) {
+    HostDevice dev;
+    if (!sizes_ok(m, n, k)) return fail("%s: size out of range", fn);
+    if (m == 0 || n == 0 || k == 0) return 0;
+    const int rc = host_device(&dev);
+    if (rc) return rc < 0 ? rc : -rc;
+    const int64_t cols = EPI == kDenseGated ? 2 * n : n;
+    if (!forward_may_cut(m, k * elem_bytes<OP>()) || stream_rows(dev, m, cols, k * elem_bytes<OP>())) return 0;
+    return 4 * split_words(plan_for<OP, EPI>(dev, m, n, k, 1, 1), m, cols);
+}
+
 DenseParams dense_params() {
     DenseParams p;
     memset(&p, 0, sizeof(p));
@@ -250,13 +305,6 @@ DenseParams dense_params() {
 }
 
 // ------------------------------------------------------------------------------ a few tokens
-// Up to 8 rows go to the streaming kernel (its floor is the weights' bytes, and it reaches 90 to 99 % of it).  For 9 to 16 its
-// activations no longer fit L1 beside the ring, so large weights go to the tile kernel.  us, streaming / tile: int8 16 x 1024
-// x 8192 6.1 / 13.3, 16 x 4096 x 4096 8.0 / 8.9, 16 x 8192 x 8192 18.6 / 17.2, 16 x 28672 x 8192 48.6 / 44.5, gated bf16
-// 16 x 14336 x 8192 86 / 76.
-bool stream_rows(int64_t m, int64_t weight_bytes) { return m <= 8 || (m <= 16 && weight_bytes <= (int64_t(32) << 20)); }
-
-
 template <bool INT8, bool GATED>
 int launch_stream(const HostDevice& dev, StreamParams p, cudaStream_t stream) {
     const int64_t groups = (p.n + 7) / 8;
@@ -364,6 +412,9 @@ cudaError_t prepare_dense_kernels() {
     PREP(gated_backward_kernel<AVE_FP4_ACT_GELU_TANH>)
     PREP(gated_backward_kernel<AVE_FP4_ACT_SILU>)
     PREP(sum_splits_kernel)
+    PREP(finish_splits_kernel<true, kDenseScaled>)
+    PREP(finish_splits_kernel<true, kDenseGated>)
+    PREP(finish_splits_kernel<false, kDenseGated>)
 #undef PREP
     return cudaSuccess;
 }
@@ -402,8 +453,13 @@ int ave_int8_quantize(const void* x_bf16, int64_t rows, int64_t k, int64_t ldx, 
     return launch_quantize<0, true>(x_bf16, rows, k, ldx, values, ldv, scales, s);
 }
 
+int64_t ave_int8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    return forward_workspace<kOpInt8, kDenseScaled>("ave_int8_gemm_workspace_bytes", m, n, k);
+}
+
 int ave_int8_gemm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, const void* b_scales,
-                  const void* bias_bf16, int activation, void* d_bf16, int64_t ldd, int64_t m, int64_t n, int64_t k, void* stream) {
+                  const void* bias_bf16, int activation, void* d_bf16, int64_t ldd, void* workspace, int64_t workspace_bytes,
+                  int64_t m, int64_t n, int64_t k, void* stream) {
     static const char* fn = "ave_int8_gemm";
     HostDevice dev;
     if (!sizes_ok(m, n, k)) return fail("%s: size out of range", fn);
@@ -423,7 +479,7 @@ int ave_int8_gemm(const void* a, int64_t lda, const void* a_scales, const void* 
     ldb = row_stride(n, k, ldb);
     ldd = row_stride(m, n, ldd);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (stream_rows(m, n * k)) {
+    if (stream_rows(dev, m, n, k)) {
         StreamParams p = stream_params(a, lda, m, n, k, activation, d_bf16, ldd);
         p.w[0] = static_cast<const uint8_t*>(b);
         p.ldw[0] = ldb;
@@ -439,12 +495,16 @@ int ave_int8_gemm(const void* a, int64_t lda, const void* a_scales, const void* 
     p.act = activation;
     p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(d_bf16);
     p.ldd = ldd;
-    return launch_dense<kOpInt8, kDenseScaled>(dev, plan_for<kOpInt8, kDenseScaled>(dev, m, n, k, 1, 1), {{a, lda}, {a, lda}}, {{b, ldb}, {b, ldb}}, m, n, k, p, s);
+    return launch_forward<kOpInt8, kDenseScaled>(dev, fn, {{a, lda}, {a, lda}}, {{b, ldb}, {b, ldb}}, m, n, k, p, workspace, workspace_bytes, s);
+}
+
+int64_t ave_int8_gemm_gated_workspace_bytes(int64_t m, int64_t f, int64_t k) {
+    return forward_workspace<kOpInt8, kDenseGated>("ave_int8_gemm_gated_workspace_bytes", m, f, k);
 }
 
 int ave_int8_gemm_gated(const void* a, int64_t lda, const void* a_scales, const void* w_gate, int64_t ld_wg, const void* gate_scales,
                         const void* w_up, int64_t ld_wu, const void* up_scales, int activation, void* d_bf16, int64_t ldd,
-                        int64_t m, int64_t f, int64_t k, void* stream) {
+                        void* workspace, int64_t workspace_bytes, int64_t m, int64_t f, int64_t k, void* stream) {
     static const char* fn = "ave_int8_gemm_gated";
     HostDevice dev;
     if (!sizes_ok(m, f, k)) return fail("%s: size out of range", fn);
@@ -466,7 +526,7 @@ int ave_int8_gemm_gated(const void* a, int64_t lda, const void* a_scales, const 
     ld_wu = row_stride(f, k, ld_wu);
     ldd = row_stride(m, f, ldd);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (stream_rows(m, 2 * f * k)) {
+    if (stream_rows(dev, m, 2 * f, k)) {
         StreamParams p = stream_params(a, lda, m, f, k, activation, d_bf16, ldd);
         p.w[0] = static_cast<const uint8_t*>(w_gate);
         p.w[1] = static_cast<const uint8_t*>(w_up);
@@ -484,12 +544,16 @@ int ave_int8_gemm_gated(const void* a, int64_t lda, const void* a_scales, const 
     p.act = activation;
     p.d[0] = p.d[1] = static_cast<__nv_bfloat16*>(d_bf16);
     p.ldd = ldd;
-    return launch_dense<kOpInt8, kDenseGated>(dev, plan_for<kOpInt8, kDenseGated>(dev, m, f, k, 1, 1), {{a, lda}, {a, lda}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, k, p, s);
+    return launch_forward<kOpInt8, kDenseGated>(dev, fn, {{a, lda}, {a, lda}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, k, p, workspace, workspace_bytes, s);
+}
+
+int64_t ave_bf16_gemm_gated_workspace_bytes(int64_t m, int64_t f, int64_t h) {
+    return forward_workspace<kOpBf16, kDenseGated>("ave_bf16_gemm_gated_workspace_bytes", m, f, h);
 }
 
 int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t ld_wg, const void* w_up, int64_t ld_wu, int activation,
                         void* d_bf16, int64_t ldd, void* gate_bf16, int64_t ld_gate, void* up_bf16, int64_t ld_up,
-                        int64_t m, int64_t f, int64_t h, void* stream) {
+                        void* workspace, int64_t workspace_bytes, int64_t m, int64_t f, int64_t h, void* stream) {
     static const char* fn = "ave_bf16_gemm_gated";
     HostDevice dev;
     if (!sizes_ok(m, f, h)) return fail("%s: size out of range", fn);
@@ -514,7 +578,7 @@ int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t 
     ld_gate = row_stride(m, f, ld_gate);
     ld_up = row_stride(m, f, ld_up);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (stream_rows(m, 4 * f * h)) {
+    if (stream_rows(dev, m, 2 * f, 2 * h)) {
         StreamParams p = stream_params(x, ldx * 2, m, f, h * 2, activation, d_bf16, ldd);
         p.w[0] = static_cast<const uint8_t*>(w_gate);
         p.w[1] = static_cast<const uint8_t*>(w_up);
@@ -534,7 +598,7 @@ int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t 
     p.up = static_cast<__nv_bfloat16*>(up_bf16);
     p.ld_gate = ld_gate;
     p.ld_up = ld_up;
-    return launch_dense<kOpBf16, kDenseGated>(dev, plan_for<kOpBf16, kDenseGated>(dev, m, f, h, 1, 1), {{x, ldx}, {x, ldx}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, h, p, s);
+    return launch_forward<kOpBf16, kDenseGated>(dev, fn, {{x, ldx}, {x, ldx}}, {{w_gate, ld_wg}, {w_up, ld_wu}}, m, f, h, p, workspace, workspace_bytes, s);
 }
 
 }  // extern "C"
@@ -545,8 +609,8 @@ namespace {
 // then touches one line), and what cuts of K in either product need.
 struct GatedBackwardPlan {
     DensePlan dx, dw;
-    int64_t ld, half, dx_floats, dw_floats;
-    int64_t bytes() const { return 2 * half + 4 * (dx_floats + dw_floats); }
+    int64_t ld, half, dx_words, dw_words;
+    int64_t bytes() const { return 2 * half + 4 * (dx_words + dw_words); }
 };
 
 GatedBackwardPlan plan_gated_backward(const HostDevice& dev, int64_t m, int64_t f, int64_t h, bool want_x, bool want_w) {
@@ -555,38 +619,32 @@ GatedBackwardPlan plan_gated_backward(const HostDevice& dev, int64_t m, int64_t 
     p.half = ceil_div(m * p.ld * 2, 256) * 256;
     if (want_x) {
         p.dx = plan_for<kOpBf16Nn, kDensePlain>(dev, m, h, f, 2, 1);
-        p.dx_floats = split_floats(p.dx, m, h);
+        p.dx_words = split_words(p.dx, m, h);
     }
     if (want_w) {
         p.dw = plan_for<kOpBf16Tn, kDensePlain>(dev, f, h, m, 1, 2);
-        p.dw_floats = split_floats(p.dw, 2 * f, h);
+        p.dw_words = split_words(p.dw, 2 * f, h);
     }
     return p;
 }
 
 struct ProductBackwardPlan {
     DensePlan da, db;
-    int64_t da_floats, db_floats;
-    int64_t bytes() const { return 4 * (da_floats + db_floats); }
+    int64_t da_words, db_words;
+    int64_t bytes() const { return 4 * (da_words + db_words); }
 };
 
 ProductBackwardPlan plan_product_backward(const HostDevice& dev, int64_t m, int64_t n, int64_t k, bool want_a, bool want_b) {
     ProductBackwardPlan p{};
     if (want_a) {
         p.da = plan_for<kOpBf16Nn, kDensePlain>(dev, m, k, n, 1, 1);
-        p.da_floats = split_floats(p.da, m, k);
+        p.da_words = split_words(p.da, m, k);
     }
     if (want_b) {
         p.db = plan_for<kOpBf16Tn, kDensePlain>(dev, n, k, m, 1, 1);
-        p.db_floats = split_floats(p.db, n, k);
+        p.db_words = split_words(p.db, n, k);
     }
     return p;
-}
-
-int check_workspace(const char* fn, const void* workspace, int64_t have, int64_t need) {
-    if (need > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || have < need))
-        return fail("%s: the workspace must be 256-byte aligned and hold %lld bytes", fn, static_cast<long long>(need));
-    return 0;
 }
 
 }  // namespace
@@ -647,8 +705,8 @@ int ave_bf16_gated_backward(const void* dd, int64_t ld_dd, const void* x, int64_
     const int64_t ld = plan.ld;
     void* d_gate = workspace;
     void* d_up = static_cast<uint8_t*>(workspace) + plan.half;
-    float* dx_partial = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + 2 * plan.half);
-    float* dw_partial = dx_partial + plan.dx_floats;
+    uint32_t* dx_partial = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(workspace) + 2 * plan.half);
+    uint32_t* dw_partial = dx_partial + plan.dx_words;
     SplitSums sums{};
     switch (activation) {
         case AVE_FP4_ACT_RELU: CHECK(launch_gated_backward<AVE_FP4_ACT_RELU>(dev, dd, ld_dd, gate, ld_gate, up, ld_up, d_gate, d_up, ld, m, f, s)); break;
@@ -716,8 +774,8 @@ int ave_bf16_gemm_backward(const void* dd, int64_t ld_dd, const void* a, int64_t
     ldb = row_stride(n, k, ldb);
     const ProductBackwardPlan plan = plan_product_backward(dev, m, n, k, da != nullptr, db != nullptr);
     CHECK(check_workspace(fn, workspace, workspace_bytes, plan.bytes()));
-    float* da_partial = static_cast<float*>(workspace);
-    float* db_partial = da_partial + plan.da_floats;
+    uint32_t* da_partial = static_cast<uint32_t*>(workspace);
+    uint32_t* db_partial = da_partial + plan.da_words;
     SplitSums sums{};
     if (da != nullptr) {
         DenseParams p = dense_params();

@@ -17,7 +17,7 @@
 // in one thread's TMEM lane.  With CTA pairs this takes no extra load: each CTA supplies half of the B tile, one of
 // them from Wg, the other from Wu.
 //
-// Structure: warps 0 and 2 TMA producers, warp 1 MMA issuer, warps 3-10 epilogue; a ring of shared-memory stages of 128 bytes of
+// Structure: warps 0 and 2 TMA producers, warp 1 MMA issuer, warps 3 and up (8 or 16 of them) epilogue; a ring of shared-memory stages of 128 bytes of
 // K per row (128-byte swizzle); two accumulators of up to 256 columns in TMEM, so a tile's epilogue runs under the next
 // tile's main loop.  The tile is 128 rows per CTA by `block_n` columns, and block_n is a run-time value: the number of
 // columns goes into the instruction descriptor, so the host picks it for whole waves (see choose_block_n).
@@ -42,8 +42,8 @@ struct DenseParams {
     int kb_stage;                    // K blocks of 128 bytes per row (64 bf16 or 128 int8 elements) in a stage: 1 or 2
     int segments;                    // 2: C = A0 B0 + A1 B1, two operand pairs of the same sizes
     int kb_split;                    // stages of K in a range
-    int splits;                      // > 1 (plain epilogue): K is cut into that many ranges whose fp32 sums go to `partial`,
-                                     // [split][result][m][n], and sum_splits_kernel adds them up
+    int splits;                      // > 1: K is cut into that many ranges whose sums (fp32, or int32 of int8) go to `partial`,
+                                     // [split][result, or gate and up][m][n]; another kernel adds them up
     int batches;                     // 2: two results, C0 from A0 and C1 from A1, B shared; tile rows of C1 follow those of C0
     int tiles_m, tiles_n;            // tiles of one result
     int block_n;                     // columns of a tile, a multiple of 8 (one CTA) or 32 (pair)
@@ -52,7 +52,7 @@ struct DenseParams {
     int a_rows;                      // rows of A in a K block: 128, or with fewer than that in all, those, to a multiple of 8
     int band;                        // tile rows per band of the schedule
     __nv_bfloat16* d[2];
-    float* partial;
+    uint32_t* partial;
     const float* a_scale;            // one per row of A
     const float* b_scale[2];         // one per row of B; gated: of Wg and Wu
     const __nv_bfloat16* bias;
@@ -69,13 +69,13 @@ template <int CG>
 struct DenseConfig {
     static constexpr int kRingBytes = 192 * 1024;        // stages of kb_stage * (a_rows + b_rows) * 128 bytes
     static constexpr int kMaxStages = 16;
-    static constexpr int kEpiWarps = 8;
-    static constexpr int kEpiBufBytes = 32 * 128;
+    static constexpr int kMaxEpiWarps = 16;
+    static constexpr int kEpiBufBytes = 32 * 64;
     static constexpr int kOffEpi = kRingBytes;
-    static constexpr int kOffBar = kOffEpi + kEpiWarps * kEpiBufBytes;
+    static constexpr int kOffBar = kOffEpi + kMaxEpiWarps * kEpiBufBytes;
     static constexpr int kOffTmemPtr = kOffBar + (2 * kMaxStages + 4) * 8;
     static constexpr int kSmemBytes = kOffTmemPtr + 16 + 1024;
-    static constexpr int kThreads = 96 + 32 * kEpiWarps;
+    static constexpr int threads(int epi_warps) { return 96 + 32 * epi_warps; }
     static constexpr int stages(int a_rows, int b_rows, int kb_stage) {
         const int n = kRingBytes / (kb_stage * (a_rows + b_rows) * 128);
         return n < kMaxStages ? n : kMaxStages;
@@ -185,8 +185,22 @@ __device__ __forceinline__ void dense_convert(const uint32_t (&v)[16], const uin
     }
 }
 
+// A warp's 2 KB transpose buffer: 64 bytes per row, 16-byte piece q of row r in place q ^ (r / 2 & 3), so that eight lanes
+// meet all banks once both when each writes its own row and when four read one row.
+__device__ __forceinline__ uint32_t piece_addr(uint32_t sbuf, int row, int q) { return sbuf + row * 64 + ((q ^ ((row >> 1) & 3)) << 4); }
+
+__device__ __forceinline__ void stage_piece(uint32_t sbuf, int row, int q, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_addr(sbuf, row, q)), "r"(w0), "r"(w1), "r"(w2), "r"(w3) : "memory");
+}
+
+__device__ __forceinline__ uint4 staged_piece(uint32_t sbuf, int row, int q) {
+    uint4 w;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(piece_addr(sbuf, row, q)) : "memory");
+    return w;
+}
+
 template <int CG, int OP, int EPI>
-__global__ void __launch_bounds__(352, 1)
+__global__ void __launch_bounds__(608, 1)
 gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constant__ CUtensorMap tm_a1,
                   const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1, const DenseParams p) {
     using Cfg = DenseConfig<CG>;
@@ -209,6 +223,7 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     const int num_tiles = tile_rows * p.tiles_n * p.splits;
     const int all_kb = p.num_kb * p.segments;
     const int stages = p.stages;
+    const int epi_warps = static_cast<int>(blockDim.x) / 32 - 3;
     const int bn_cta = p.block_n / CG;                            // columns of the tile whose B one CTA loads
     const int b_bytes = p.b_rows * 128;                           // whole 1 KB swizzle groups
     const int a_bytes = p.a_rows * 128;
@@ -234,7 +249,7 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(bar_tfull + a * 8, 1);
-            mbar_init(bar_tempty + a * 8, Cfg::kEpiWarps * CG);
+            mbar_init(bar_tempty + a * 8, epi_warps * CG);
         }
         fence_mbar_init();
     }
@@ -392,8 +407,8 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     } else {
         // --------------------------------------------------------------- epilogue
         const int quad = warp & 3;             // TMEM lane quadrant this warp may access
-        const int half = (warp - 3) >> 2;      // takes every second group of `unit` result columns
-        const int unit = (out_cols > 64) ? 64 : 32;
+        const int part = (warp - 3) >> 2;      // of the 2 or 4 warps of a quadrant, which take groups of 32 result columns in turn
+        const int parts = epi_warps >> 2;
         const uint32_t sbuf = smem_base + Cfg::kOffEpi + (warp - 3) * Cfg::kEpiBufBytes;
         const uint32_t tempty0 = (CG == 2) ? mapa_shared(bar_tempty, 0) : bar_tempty;
         const int results = (kGated && p.gate != nullptr) ? 3 : 1;
@@ -410,48 +425,42 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
             // the row's scale and the first columns' scales and bias come while the products still run
             if constexpr (kInt8) sa = (row0 + lane < p.m) ? __ldg(p.a_scale + row0 + lane) : 0.0f;
             ColumnTerms<kInt8, EPI> terms;
-            load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col0 + half * unit, p.n);
+            load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col0 + part * 32, p.n);
             if (!mbar_wait(bar_tfull + acc * 8, acc_phase)) {
                 if (lane == 0) atomicCAS(p.status, 0, 103);
                 break;
             }
             tcgen05_fence_after();
             const uint32_t t_acc = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * 256;
-            if (EPI == kDensePlain && p.splits > 1) {
-                // fp32 sums of a K range: 32 rows x 32 columns at a time through the same transpose
-                float* base = p.partial + (static_cast<long long>(split * p.batches + (second ? 1 : 0)) * p.m) * p.n;
-                for (int c0 = half * 32; c0 < out_cols; c0 += 64) {
-                    uint32_t v[32];
-                    tmem_ld_32x32b_x32(t_acc + c0, v);
-                    tmem_ld_wait();
+            if (p.splits > 1) {
+                // sums of a K range, 16 columns (64 bytes) at a time
+                constexpr int kSlabs = kGated ? 2 : 1;
+                for (int slab = 0; slab < kSlabs; ++slab) {
+                    uint32_t* base = p.partial + static_cast<long long>(split * (kGated ? 2 : p.batches) + (kGated ? slab : second ? 1 : 0)) * p.m * p.n;
+                    for (int c0 = part * 16; c0 < out_cols; c0 += parts * 16) {
+                        uint32_t v[16];
+                        tmem_ld_32x32b_x16(t_acc + slab * out_cols + c0, v);
+                        tmem_ld_wait();
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        const uint32_t addr = sbuf + lane * 128 + ((q ^ (lane & 7)) << 4);
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[4 * q]), "r"(v[4 * q + 1]),
-                                     "r"(v[4 * q + 2]), "r"(v[4 * q + 3])
-                                     : "memory");
-                    }
-                    __syncwarp();
-                    const int q = lane & 7;
-                    const int c = c0 + q * 4;
-                    const bool col_ok = (c < out_cols) && (col0 + c < p.n);
+                        for (int q = 0; q < 4; ++q) stage_piece(sbuf, lane, q, v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                        __syncwarp();
+                        const int c = c0 + (lane & 3) * 4;
+                        const bool col_ok = (c < out_cols) && (col0 + c < p.n);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int rr = i * 4 + (lane >> 3);
-                        const uint32_t addr = sbuf + rr * 128 + ((q ^ (rr & 7)) << 4);
-                        uint32_t w0, w1, w2, w3;
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3) : "r"(addr) : "memory");
-                        if (col_ok && row0 + rr < p.m)
-                            *reinterpret_cast<uint4*>(base + static_cast<long long>(row0 + rr) * p.n + col0 + c) = make_uint4(w0, w1, w2, w3);
+                        for (int i = 0; i < 4; ++i) {
+                            const int rr = i * 8 + (lane >> 2);
+                            const uint4 w = staged_piece(sbuf, rr, lane & 3);
+                            if (col_ok && row0 + rr < p.m) *reinterpret_cast<uint4*>(base + static_cast<long long>(row0 + rr) * p.n + col0 + c) = w;
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             } else
-            for (int c0 = half * unit; c0 < out_cols; c0 += 2 * unit) {
-                const int c1 = min(c0 + unit, out_cols);
+            for (int c0 = part * 32; c0 < out_cols; c0 += parts * 32) {
+                const int c1 = min(c0 + 32, out_cols);
                 for (int r = 0; r < results; ++r) {
-                    // 32 rows x up to 64 columns through a swizzled transpose: lane = row, 16-byte chunk q of a row lives at
-                    // chunk q ^ (row & 7); a row's part of the result is then stored by neighbouring lanes
+                    // 32 rows x up to 32 columns through a transpose in shared memory, so that a row's part of the result is
+                    // stored by neighbouring lanes
 #pragma unroll 1
                     for (int c = c0; c < c1; c += 16) {
                         uint32_t v[16], u[16], w[8];
@@ -470,34 +479,25 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
                             }
                         }
                         if constexpr (kInt8) {      // the next 16 columns' terms: in this group, or the first of the next one
-                            const int next = (c + 16 < c1) ? c + 16 : c0 + 2 * unit;
+                            const int next = (c + 16 < c1) ? c + 16 : c0 + parts * 32;
                             load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col0 + next, p.n);
                         }
                         const int q0 = (c - c0) / 8;
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const uint32_t addr = sbuf + lane * 128 + (((q0 + q) ^ (lane & 7)) << 4);
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[4 * q]), "r"(w[4 * q + 1]),
-                                         "r"(w[4 * q + 2]), "r"(w[4 * q + 3])
-                                         : "memory");
-                        }
+                        for (int q = 0; q < 2; ++q) stage_piece(sbuf, lane, q0 + q, w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
                     }
                     __syncwarp();
                     __nv_bfloat16* d = p.d[second ? 1 : 0];
                     long long ld = p.ldd;
                     if (kGated && r == 1) { d = p.gate; ld = p.ld_gate; }
                     if (kGated && r == 2) { d = p.up; ld = p.ld_up; }
-                    const int q = lane & 7;
-                    const int c = c0 + q * 8;
+                    const int c = c0 + (lane & 3) * 8;
                     const bool col_ok = (c < c1) && (col0 + c < p.n);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int rr = i * 4 + (lane >> 3);
-                        const uint32_t addr = sbuf + rr * 128 + ((q ^ (rr & 7)) << 4);
-                        uint32_t w0, w1, w2, w3;
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3) : "r"(addr) : "memory");
-                        if (col_ok && row0 + rr < p.m)
-                            __stcs(reinterpret_cast<uint4*>(d + (row0 + rr) * ld + col0 + c), make_uint4(w0, w1, w2, w3));
+                    for (int i = 0; i < 4; ++i) {
+                        const int rr = i * 8 + (lane >> 2);
+                        const uint4 w = staged_piece(sbuf, rr, lane & 3);
+                        if (col_ok && row0 + rr < p.m) __stcs(reinterpret_cast<uint4*>(d + (row0 + rr) * ld + col0 + c), w);
                     }
                     __syncwarp();
                 }
@@ -518,9 +518,9 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     if (warp == 1) tmem_dealloc<CG>(tmem_base, 512);
 }
 
-// Adds up the K ranges of up to three results and rounds once: one thread takes 8 columns of a row.
+// Adds up the K ranges of up to three plain results and rounds once: one thread takes 8 columns of a row.
 struct SplitSum {
-    const float* partial;        // first range; `stride` floats to the next
+    const uint32_t* partial;     // first range; `stride` words to the next
     long long stride;
     __nv_bfloat16* d;
     long long ldd;
@@ -532,6 +532,18 @@ struct SplitSums {
     SplitSum job[3];
 };
 
+// 8 columns of a K range added to the sums so far
+template <bool INT8>
+__device__ __forceinline__ void add_range(uint32_t (&acc)[8], const uint32_t* src) {
+    const uint4 lo = __ldcs(reinterpret_cast<const uint4*>(src)), hi = __ldcs(reinterpret_cast<const uint4*>(src) + 1);
+    const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (INT8) acc[i] += w[i];
+        else acc[i] = __float_as_uint(__uint_as_float(acc[i]) + __uint_as_float(w[i]));
+    }
+}
+
 __global__ void __launch_bounds__(256)
 sum_splits_kernel(const SplitSums p) {
     pdl_launch_dependents();
@@ -540,19 +552,58 @@ sum_splits_kernel(const SplitSums p) {
     for (int j = 0; j < 3; ++j) {
         const SplitSum& s = p.job[j];
         for (long long i = blockIdx.x * 256ll + threadIdx.x; i < s.pieces; i += gridDim.x * 256ll) {
-            float acc[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
-            for (int r = 0; r < s.splits; ++r) {
-                const float4* src = reinterpret_cast<const float4*>(s.partial + r * s.stride + i * 8);
-                const float4 lo = __ldcs(src), hi = __ldcs(src + 1);
-                acc[0] += lo.x; acc[1] += lo.y; acc[2] += lo.z; acc[3] += lo.w;
-                acc[4] += hi.x; acc[5] += hi.y; acc[6] += hi.z; acc[7] += hi.w;
-            }
+            uint32_t acc[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+            for (int r = 0; r < s.splits; ++r) add_range<false>(acc, s.partial + r * s.stride + i * 8);
             const long long row = i / s.n8;
             const long long col = (i - row * s.n8) * 8;
-            *reinterpret_cast<uint4*>(s.d + row * s.ldd + col) =
-                make_uint4(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]), pack_bf16(acc[4], acc[5]), pack_bf16(acc[6], acc[7]));
+            uint32_t w[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w[c] = pack_bf16(__uint_as_float(acc[2 * c]), __uint_as_float(acc[2 * c + 1]));
+            *reinterpret_cast<uint4*>(s.d + row * s.ldd + col) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// The same for a scaled or gated result, with the tile kernel's epilogue.  That takes 16 columns; a thread here has 8, and the other
+// half of its work falls away in the compiler.
+template <bool INT8, int EPI>
+__global__ void __launch_bounds__(256)
+finish_splits_kernel(const DenseParams p) {
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    const int n8 = p.n / 8;
+    const long long pieces = static_cast<long long>(p.m) * n8;
+    const long long slab = static_cast<long long>(p.m) * p.n;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < pieces; i += gridDim.x * 256ll) {
+        const int row = static_cast<int>(i / n8);
+        const int col = static_cast<int>(i - static_cast<long long>(row) * n8) * 8;
+        uint32_t g[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u}, u[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+        for (int r = 0; r < p.splits; ++r) {
+            const uint32_t* src = p.partial + (EPI == kDenseGated ? 2 * r : r) * slab + i * 8;
+            add_range<INT8>(g, src);
+            if constexpr (EPI == kDenseGated) add_range<INT8>(u, src + slab);
+        }
+        const float sa = INT8 ? __ldg(p.a_scale + row) : 1.0f;
+        ColumnTerms<INT8, EPI> terms;
+        load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col, p.n);
+        uint32_t v16[16], u16[16], w[8];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) { v16[c] = g[c & 7]; u16[c] = u[c & 7]; }
+        switch (p.act) {
+            case AVE_FP4_ACT_RELU: dense_convert<INT8, EPI, AVE_FP4_ACT_RELU>(v16, u16, w, sa, terms); break;
+            case AVE_FP4_ACT_GELU: dense_convert<INT8, EPI, AVE_FP4_ACT_GELU>(v16, u16, w, sa, terms); break;
+            case AVE_FP4_ACT_GELU_TANH: dense_convert<INT8, EPI, AVE_FP4_ACT_GELU_TANH>(v16, u16, w, sa, terms); break;
+            case AVE_FP4_ACT_SILU: dense_convert<INT8, EPI, AVE_FP4_ACT_SILU>(v16, u16, w, sa, terms); break;
+            default: dense_convert<INT8, EPI, AVE_FP4_ACT_NONE>(v16, u16, w, sa, terms); break;
+        }
+        *reinterpret_cast<uint4*>(p.d[0] + row * p.ldd + col) = make_uint4(w[0], w[1], w[2], w[3]);
+        if constexpr (EPI == kDenseGated && !INT8) {
+            if (p.gate != nullptr) {
+                dense_convert<false, kDensePlain, AVE_FP4_ACT_NONE>(v16, v16, w, 1.0f, ColumnTerms<false, kDensePlain>{});
+                *reinterpret_cast<uint4*>(p.gate + row * p.ld_gate + col) = make_uint4(w[0], w[1], w[2], w[3]);
+                dense_convert<false, kDensePlain, AVE_FP4_ACT_NONE>(u16, u16, w, 1.0f, ColumnTerms<false, kDensePlain>{});
+                *reinterpret_cast<uint4*>(p.up + row * p.ld_up + col) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
     }
 }

@@ -50,8 +50,10 @@ def gemm_gated_transposed_b(x: torch.Tensor, W_gate: torch.Tensor, W_up: torch.T
         gate = torch.empty(m, f, dtype=torch.bfloat16, device=x.device)
         up = torch.empty(m, f, dtype=torch.bfloat16, device=x.device)
     if m and f:
+        hold, workspace, need = _dense.forward_workspace("ave_bf16_gemm_gated", x.device, m, f, h, 2 * h)
         _dense.call("ave_bf16_gemm_gated", x.device, x.data_ptr(), ldx, W_gate.data_ptr(), ldg, W_up.data_ptr(), ldu, act,
-                    out.data_ptr(), ldd, gate.data_ptr() if save else None, f, up.data_ptr() if save else None, f, m, f, h)
+                    out.data_ptr(), ldd, gate.data_ptr() if save else None, f, up.data_ptr() if save else None, f,
+                    workspace, need, m, f, h)
     return (out, gate, up) if save else out
 
 

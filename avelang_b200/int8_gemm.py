@@ -108,8 +108,10 @@ def gemm_int8_transposed_b(A: Int8Operand, B: Int8Operand, out: torch.Tensor | N
         _dense.vector(bias, "bias", torch.bfloat16, n, dev)
     out, ldd = _dense.result(out, "out", m, n, dev)
     if m and n:
+        hold, workspace, need = _dense.forward_workspace("ave_int8_gemm", dev, m, n, k, k)
         _dense.call("ave_int8_gemm", dev, A.values.data_ptr(), lda, A.scales.data_ptr(), B.values.data_ptr(), ldb, B.scales.data_ptr(),
-                    None if bias is None else bias.data_ptr(), act, out.data_ptr(), ldd, m, n, k)
+                    None if bias is None else bias.data_ptr(), act, out.data_ptr(), ldd,
+                    workspace, need, m, n, k)
     return out
 
 
@@ -130,7 +132,8 @@ def gemm_int8_gated_transposed_b(A: Int8Operand, W_gate: Int8Operand, W_up: Int8
     _dense.multiple(f, "F", 8)
     out, ldd = _dense.result(out, "out", m, f, dev)
     if m and f:
+        hold, workspace, need = _dense.forward_workspace("ave_int8_gemm_gated", dev, m, f, k, k)
         _dense.call("ave_int8_gemm_gated", dev, A.values.data_ptr(), lda, A.scales.data_ptr(), W_gate.values.data_ptr(), ldg,
                     W_gate.scales.data_ptr(), W_up.values.data_ptr(), ldu, W_up.scales.data_ptr(), act, out.data_ptr(), ldd,
-                    m, f, k)
+                    workspace, need, m, f, k)
     return out

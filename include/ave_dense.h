@@ -34,22 +34,30 @@ int ave_int8_quantize(const void* x_bf16, int64_t rows, int64_t k, int64_t ldx, 
 /*
  * D (m, n) bf16 = act(a_scales[row] * b_scales[col] * (A (m, k) B (n, k)^T) + bias[col]) on int8 operands; the integer sums
  * are exact (k <= AVE_INT8_MAX_K), the rest is fp32, rounded to bf16 once.  k % 16 == 0, n % 8 == 0.  bias_bf16 may be NULL.
+ * `workspace` (here and in the two gated products): the bytes that the _workspace_bytes function gives for these sizes on the
+ * current device, 256-byte aligned; 0 of them whenever m <= 8 or a row of K is shorter than AVE_DENSE_MIN_CUT_BYTES, and for most
+ * other sizes.  It holds partial sums during the call and no state between calls.
  */
+#define AVE_DENSE_MIN_CUT_BYTES 4096
+int64_t ave_int8_gemm_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int ave_int8_gemm(const void* a, int64_t lda, const void* a_scales, const void* b, int64_t ldb, const void* b_scales,
-                  const void* bias_bf16, int activation, void* d_bf16, int64_t ldd, int64_t m, int64_t n, int64_t k, void* stream);
+                  const void* bias_bf16, int activation, void* d_bf16, int64_t ldd, void* workspace, int64_t workspace_bytes,
+                  int64_t m, int64_t n, int64_t k, void* stream);
 
-/* D (m, f) bf16 = act(A Wg^T) * (A Wu^T), int8 operands with scales as above, one kernel. */
+/* D (m, f) bf16 = act(A Wg^T) * (A Wu^T), int8 operands with scales as above, one pass. */
+int64_t ave_int8_gemm_gated_workspace_bytes(int64_t m, int64_t f, int64_t k);
 int ave_int8_gemm_gated(const void* a, int64_t lda, const void* a_scales, const void* w_gate, int64_t ld_wg, const void* gate_scales,
                         const void* w_up, int64_t ld_wu, const void* up_scales, int activation, void* d_bf16, int64_t ldd,
-                        int64_t m, int64_t f, int64_t k, void* stream);
+                        void* workspace, int64_t workspace_bytes, int64_t m, int64_t f, int64_t k, void* stream);
 
 /*
  * D (m, f) = act(X Wg^T) * (X Wu^T) on bf16: X (m, h), Wg and Wu (f, h); both products in one kernel, fp32 up to the one
  * rounding.  gate_bf16 and up_bf16 (both or neither NULL) receive X Wg^T and X Wu^T, for the backward pass.  h % 8 == 0, f % 8 == 0.
  */
+int64_t ave_bf16_gemm_gated_workspace_bytes(int64_t m, int64_t f, int64_t h);
 int ave_bf16_gemm_gated(const void* x, int64_t ldx, const void* w_gate, int64_t ld_wg, const void* w_up, int64_t ld_wu, int activation,
                         void* d_bf16, int64_t ldd, void* gate_bf16, int64_t ld_gate, void* up_bf16, int64_t ld_up,
-                        int64_t m, int64_t f, int64_t h, void* stream);
+                        void* workspace, int64_t workspace_bytes, int64_t m, int64_t f, int64_t h, void* stream);
 
 /*
  * Backward pass of ave_bf16_gemm_gated from dD (m, f) and the kept products gate and up:

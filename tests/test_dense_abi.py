@@ -95,15 +95,15 @@ def test_c_entries_refuse_before_any_launch(lib):
     _refused(lib, q(P, 4, 32, 32, ctypes.c_void_p(4100), 32, P, None), "values is null or not 16-byte aligned")
     _refused(lib, q(None, 4, 32, 32, P, 32, P, None), "x is null")
     _refused(lib, q(P, -1, 32, 32, P, 32, P, None), "size out of range")
-    _refused(lib, g(P, 64, P, P, 64, P, None, 0, P, 12, 4, 12, 64, None), "N must be a multiple of 8")
-    _refused(lib, g(P, 64, P, P, 64, P, None, 5, P, 16, 4, 16, 64, None), "unknown activation 5")
-    _refused(lib, g(P, 131072, P, P, 131072, P, None, 0, P, 16, 4, 16, 131072, None), "at most 131056")
-    _refused(lib, g(P, 64, None, P, 64, P, None, 0, P, 16, 4, 16, 64, None), "the scales of A")
-    _refused(lib, g(P, 64, P, P, 64, P, ctypes.c_void_p(4098), 0, P, 16, 4, 16, 64, None), "the bias")
-    _refused(lib, g(P, 64, P, P, 64, P, None, 0, P, 20, 4, 16, 64, None), "row stride of D")
-    _refused(lib, lib.ave_int8_gemm_gated(P, 64, P, P, 64, P, P, 56, P, 4, P, 16, 4, 16, 64, None), "row stride of W_up")
-    _refused(lib, lib.ave_bf16_gemm_gated(P, 64, P, 64, P, 64, 4, P, 16, P, 16, None, 16, 4, 16, 64, None), "kept together")
-    _refused(lib, lib.ave_bf16_gemm_gated(P, 64, P, 64, P, 64, 4, P, 16, None, 16, None, 16, 4, 16, 60, None), "H must be a positive multiple of 8")
+    _refused(lib, g(P, 64, P, P, 64, P, None, 0, P, 12, None, 0, 4, 12, 64, None), "N must be a multiple of 8")
+    _refused(lib, g(P, 64, P, P, 64, P, None, 5, P, 16, None, 0, 4, 16, 64, None), "unknown activation 5")
+    _refused(lib, g(P, 131072, P, P, 131072, P, None, 0, P, 16, None, 0, 4, 16, 131072, None), "at most 131056")
+    _refused(lib, g(P, 64, None, P, 64, P, None, 0, P, 16, None, 0, 4, 16, 64, None), "the scales of A")
+    _refused(lib, g(P, 64, P, P, 64, P, ctypes.c_void_p(4098), 0, P, 16, None, 0, 4, 16, 64, None), "the bias")
+    _refused(lib, g(P, 64, P, P, 64, P, None, 0, P, 20, None, 0, 4, 16, 64, None), "row stride of D")
+    _refused(lib, lib.ave_int8_gemm_gated(P, 64, P, P, 64, P, P, 56, P, 4, P, 16, None, 0, 4, 16, 64, None), "row stride of W_up")
+    _refused(lib, lib.ave_bf16_gemm_gated(P, 64, P, 64, P, 64, 4, P, 16, P, 16, None, 16, None, 0, 4, 16, 64, None), "kept together")
+    _refused(lib, lib.ave_bf16_gemm_gated(P, 64, P, 64, P, 64, 4, P, 16, None, 16, None, 16, None, 0, 4, 16, 60, None), "H must be a positive multiple of 8")
     back = lib.ave_bf16_gated_backward
     assert lib.ave_bf16_gated_backward_workspace_bytes(-1, 16, 64, 1, 1) < 0 and lib.ave_bf16_gemm_backward_workspace_bytes(4, 16, -64, 1, 1) < 0
     ok = [P, 16, P, 64, P, 64, P, 64, P, 16, P, 16, 4, P, 64, P, P, 64]

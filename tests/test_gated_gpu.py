@@ -306,3 +306,14 @@ print("fine")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "fine" in run.stdout, run.stdout + run.stderr
+
+
+@pytest.mark.parametrize("m,f,h", [(28, 1016, 6712), (40, 64, 8200), (300, 264, 4104), (17, 2056, 5008), (129, 520, 2048)])
+def test_forward_with_long_sums(cuda_device, m, f, h):
+    x, wg, wu = _block(cuda_device, m, f, h)
+    for activation in ACTS:
+        kept = ave.gemm_gated_transposed_b(x, wg, wu, activation=activation, save=True)
+        for got, w, what in zip(kept, D.gated(x, wg, wu, activation), ("out", "gate", "up")):
+            D.check(got, w, f"{activation} {what}")
+        assert torch.equal(kept[0], ave.gemm_gated_transposed_b(x, wg, wu, activation=activation))
+    ave.check_device_status(cuda_device)

@@ -214,17 +214,35 @@ def test_serving_block_on_a_side_stream_and_in_graphs(cuda_device, m):
     ave.check_device_status(cuda_device)
 
 
-def test_nine_to_sixteen_rows_on_large_weights(cuda_device):
-    """More than 32 MB of weights go to the tile kernel from 9 rows on, less to the streaming kernel: both sides of the rule."""
-    for n, k in ((8456, 4112), (7912, 4112)):
+def test_both_sides_of_the_streaming_rule(cuda_device):
+    """Few rows go to the streaming kernel or to the tile kernel by the number of weight rows and the length of K."""
+    for n, k in ((2360, 4112), (2400, 4112), (4728, 272), (4760, 272), (4760, 8192), (4760, 8208)):
         b = _ints(cuda_device, n, k, 2)
-        for m in (8, 9, 16):
+        for m in (1, 8, 9, 16):
             a = _ints(cuda_device, m, k, m)
             D.check(ave.gemm_int8_transposed_b(a, b, activation="silu"), D.int8_gemm(a, b, None, "silu"), f"{m}x{n}x{k}")
-    wg, wu = _ints(cuda_device, 4264, 4112, 5), _ints(cuda_device, 4264, 4112, 6)
-    for m in (9, 13, 16):
-        a = _ints(cuda_device, m, 4112, m)
-        D.check(ave.gemm_int8_gated_transposed_b(a, wg, wu), D.int8_gated(a, wg, wu, "silu"), f"gated {m}")
+    for f in (1176, 1192, 2392):
+        wg, wu = _ints(cuda_device, f, 4112, 5), _ints(cuda_device, f, 4112, 6)
+        for m in (3, 9, 13, 16):
+            a = _ints(cuda_device, m, 4112, m)
+            D.check(ave.gemm_int8_gated_transposed_b(a, wg, wu), D.int8_gated(a, wg, wu, "silu"), f"gated {m}x{f}")
+    ave.check_device_status(cuda_device)
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 64, 16384), (17, 3000, 8208), (300, 264, 12304), (890, 512, 11120), (130, 1032, 4096), (9, 2504, 16400)])
+def test_long_sums_of_few_tiles(cuda_device, m, n, k):
+    """K cut into ranges: the integer sums stay exact, whatever the cut."""
+    a, b, c = _ints(cuda_device, m, k, 1), _ints(cuda_device, n, k, 2), _ints(cuda_device, n, k, 3)
+    bias = _randn(cuda_device, 1, n, 3)[0]
+    for activation in ACTS:
+        D.check(ave.gemm_int8_transposed_b(a, b, bias=bias, activation=activation), D.int8_gemm(a, b, bias, activation), f"{activation}")
+        D.check(ave.gemm_int8_gated_transposed_b(a, b, c, activation=activation), D.int8_gated(a, b, c, activation), f"gated {activation}")
+    hold = torch.full((m + 2, n + 32), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    out = hold[1:m + 1, 16:n + 16]
+    ave.gemm_int8_transposed_b(a, b, out=out)
+    assert torch.equal(out, ave.gemm_int8_transposed_b(a, b))
+    out.fill_(7.0)
+    assert (hold == 7.0).all()
     ave.check_device_status(cuda_device)
 
 
