@@ -149,7 +149,7 @@ DensePlan plan_dense(int sms, int64_t m, int64_t cols, int64_t k_bytes, int segm
             }
         }
     }
-    best.stages = DenseConfig<1>::stages(best.a_rows, best.b_rows, best.kb_stage);
+    best.stages = DenseConfig::stages(best.a_rows, best.b_rows, best.kb_stage);
     return best;
 }
 
@@ -159,8 +159,8 @@ constexpr int64_t elem_bytes() { return OP == kOpInt8 ? 1 : 2; }
 // Forward products cut K only from here on: below they ask for no workspace, and a caller need not ask.
 bool forward_may_cut(int64_t m, int64_t k_bytes) { return m > 8 && k_bytes >= AVE_DENSE_MIN_CUT_BYTES; }
 
-// m, n: sizes of one result; k: sum length of one segment.  A plan depends on the sizes alone and takes a few microseconds
-// to find, as long as a small product runs: each host thread keeps the last ones it made.
+// m, n: sizes of one result; k: sum length of one segment.  A plan depends on the sizes alone and takes as long to find as a
+// small product runs, a few microseconds: each host thread keeps the last ones it made.
 template <int OP, int EPI>
 DensePlan plan_for(const HostDevice& dev, int64_t m, int64_t n, int64_t k, int segments, int batches) {
     struct Slot {
@@ -188,7 +188,7 @@ DensePlan plan_for(const HostDevice& dev, int64_t m, int64_t n, int64_t k, int s
 template <int CG, int OP, int EPI>
 int launch_dense_cg(const HostDevice& dev, const DensePlan& plan, const Operand (&a)[2], const Operand (&b)[2], int64_t m, int64_t n, int64_t k,
                     DenseParams p, cudaStream_t stream) {
-    using Cfg = DenseConfig<CG>;
+    using Cfg = DenseConfig;
     constexpr bool kAMn = (OP == kOpBf16Tn), kBMn = (OP == kOpBf16Nn || OP == kOpBf16Tn);
     constexpr int64_t kElem = elem_bytes<OP>();
     const int out_cols = (EPI == kDenseGated) ? plan.block_n / 2 : plan.block_n;
@@ -371,7 +371,7 @@ namespace avefp4 {
 cudaError_t prepare_dense_kernels() {
     cudaError_t e;
 #define PREP(CG, OP, EPI)                                                                                                              \
-    if ((e = cudaFuncSetAttribute(gemm_dense_kernel<CG, OP, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, DenseConfig<CG>::kSmemBytes)) != cudaSuccess) \
+    if ((e = cudaFuncSetAttribute(gemm_dense_kernel<CG, OP, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, DenseConfig::kSmemBytes)) != cudaSuccess) \
         return e;
     PREP(1, kOpInt8, kDenseScaled)
     PREP(2, kOpInt8, kDenseScaled)

@@ -17,10 +17,19 @@
 // in one thread's TMEM lane.  With CTA pairs this takes no extra load: each CTA supplies half of the B tile, one of
 // them from Wg, the other from Wu.
 //
-// Structure: warps 0 and 2 TMA producers, warp 1 MMA issuer, warps 3 and up (8 or 16 of them) epilogue; a ring of shared-memory stages of 128 bytes of
-// K per row (128-byte swizzle); two accumulators of up to 256 columns in TMEM, so a tile's epilogue runs under the next
-// tile's main loop.  The tile is 128 rows per CTA by `block_n` columns, and block_n is a run-time value: the number of
-// columns goes into the instruction descriptor, so the host picks it for whole waves (see choose_block_n).
+// Structure: warps 0 and 2 TMA producers (A and B), warp 1 MMA issuer, 8 or 16 epilogue warps; a ring of shared-memory stages
+// of one or two K blocks of 128 bytes per row (128-byte swizzle); two accumulators of up to 256 columns in TMEM, so a tile's
+// epilogue runs under the next tile's main loop.  The tile is 128 rows per CTA (one, or a pair on one instruction) by block_n
+// columns, and block_n is a run-time value: the number of columns goes into the instruction descriptor, so the host picks
+// it, and cuts of K for long sums of few tiles, by an estimate of the launch's clocks (plan_dense in ave_dense_api.cu).
+//
+// Measured on a B200, one launch, operands not in L2 (burst; back to back the power cap takes some 15 %): int8 8192^3 327 us
+// (3.36 POP/s, twice the rate of cuBLAS in bf16), gated int8 4096 x 28672 x 8192 1.09 ms (3.53 POP/s), gated bf16 4096 x 16384 x
+// 4096 665 us (1.65 PFLOP/s), C = A B and C = A^T B of 8192 x 4096 x 16384 0.70 and 0.69 ms (1.57 PFLOP/s): bound by the tensor
+// pipe.  int8 16 x 28672 x 8192 42.5 us (5.5 TB/s) and gated bf16 128 x 14336 x 8192 82 us (5.7 TB/s): bound by reading the weights.
+// With a K block of less than 256 columns the operands' way from L2 is the limit (50 to 64 bytes a clock and SM), and below
+// some 10 us the launch is: 0.8 us until the first operands are there, 0.3 until the first accumulator, 0.5 to 1 for the epilogue
+// and 0.3 to 0.7 to leave.
 //
 // An MN-major operand tile is kept as boxes of 64 elements (one swizzled 128-byte row) x 64 K rows, 8 KB each: the
 // matrix descriptor steps 8 KB from one box to the next along MN (leading offset) and 1 KB from one group of eight
@@ -65,7 +74,6 @@ struct DenseParams {
     int* status;
 };
 
-template <int CG>
 struct DenseConfig {
     static constexpr int kRingBytes = 192 * 1024;        // stages of kb_stage * (a_rows + b_rows) * 128 bytes
     static constexpr int kMaxStages = 16;
@@ -138,28 +146,34 @@ __device__ __forceinline__ void dense_tile(int t, int rows, int cols, int band, 
     tn = r / in_band;
 }
 
-// 16 accumulator columns of this thread's row -> 8 words of bf16 pairs.  `col` is the first one's column in the result.
-// (16 and not more at a time keeps the code of five activations small: a short launch runs it from a cold instruction cache.)
+// What the epilogue needs of 16 columns beside their accumulators.
 template <bool INT8, int EPI>
 struct ColumnTerms {
     float4 s0[INT8 ? 4 : 1], s1[INT8 && EPI == kDenseGated ? 4 : 1];
-    uint2 bias[EPI == kDenseScaled ? 4 : 1];
+    uint4 bias[EPI == kDenseScaled ? 2 : 1];
 };
 
-// Scales and bias of 16 columns from `col` on; the ones past the last column stand in for any.  n is a multiple of 8.
+// Scales and bias of 16 columns from `col` on, in two halves: n is a multiple of 8, and where a half lies past the last column any
+// other stands in for it.
 template <bool INT8, int EPI>
 __device__ __forceinline__ void load_terms(ColumnTerms<INT8, EPI>& t, const float* sb0, const float* sb1, const __nv_bfloat16* bias, int col, int n) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int at = min(col + 4 * q, n - 4);
+    for (int h = 0; h < 2; ++h) {
+        const int at = min(col + 8 * h, n - 8);
         if constexpr (INT8) {
-            t.s0[q] = __ldg(reinterpret_cast<const float4*>(sb0 + at));
-            if constexpr (EPI == kDenseGated) t.s1[q] = __ldg(reinterpret_cast<const float4*>(sb1 + at));
+            t.s0[2 * h] = __ldg(reinterpret_cast<const float4*>(sb0 + at));
+            t.s0[2 * h + 1] = __ldg(reinterpret_cast<const float4*>(sb0 + at) + 1);
+            if constexpr (EPI == kDenseGated) {
+                t.s1[2 * h] = __ldg(reinterpret_cast<const float4*>(sb1 + at));
+                t.s1[2 * h + 1] = __ldg(reinterpret_cast<const float4*>(sb1 + at) + 1);
+            }
         }
-        if constexpr (EPI == kDenseScaled) t.bias[q] = (bias != nullptr) ? __ldg(reinterpret_cast<const uint2*>(bias + at)) : make_uint2(0u, 0u);
+        if constexpr (EPI == kDenseScaled) t.bias[h] = (bias != nullptr) ? __ldg(reinterpret_cast<const uint4*>(bias + at)) : make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
+// 16 accumulator columns of this thread's row -> 8 words of bf16 pairs.  (16 and not more at a time keeps the code of five
+// activations small: a short launch runs it from a cold instruction cache.)
 template <bool INT8, int EPI, int ACT>
 __device__ __forceinline__ void dense_convert(const uint32_t (&v)[16], const uint32_t (&u)[16], uint32_t (&w)[8], float sa,
                                               const ColumnTerms<INT8, EPI>& t) {
@@ -168,14 +182,17 @@ __device__ __forceinline__ void dense_convert(const uint32_t (&v)[16], const uin
         float c0[4], c1[4], b[4], y[4];
         if constexpr (INT8) { c0[0] = t.s0[q].x; c0[1] = t.s0[q].y; c0[2] = t.s0[q].z; c0[3] = t.s0[q].w; }
         if constexpr (INT8 && EPI == kDenseGated) { c1[0] = t.s1[q].x; c1[1] = t.s1[q].y; c1[2] = t.s1[q].z; c1[3] = t.s1[q].w; }
-        if constexpr (EPI == kDenseScaled) { b[0] = bf16_lo(t.bias[q].x); b[1] = bf16_hi(t.bias[q].x); b[2] = bf16_lo(t.bias[q].y); b[3] = bf16_hi(t.bias[q].y); }
+        if constexpr (EPI == kDenseScaled) {
+            const uint32_t lo = (q & 1) ? t.bias[q >> 1].z : t.bias[q >> 1].x, hi = (q & 1) ? t.bias[q >> 1].w : t.bias[q >> 1].y;
+            b[0] = bf16_lo(lo); b[1] = bf16_hi(lo); b[2] = bf16_lo(hi); b[3] = bf16_hi(hi);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             // int32 -> fp32 rounds to nearest: 2^-24 of the sum, far below the one rounding to bf16.  The channel's scale comes
             // first: weights are of ordinary size, so the product with a large token's scale overflows only if the result does.
             float g = __uint_as_float(v[4 * q + i]);
-            if constexpr (INT8) g = __int2float_rn(static_cast<int>(v[4 * q + i])) * c0[i] * sa;
-            if constexpr (EPI == kDenseScaled) g += b[i];
+            if constexpr (INT8 && EPI == kDenseScaled) g = fmaf(__int2float_rn(static_cast<int>(v[4 * q + i])) * c0[i], sa, b[i]);
+            else if constexpr (INT8) g = __int2float_rn(static_cast<int>(v[4 * q + i])) * c0[i] * sa;
             y[i] = act_value<ACT>(g);
             if constexpr (EPI == kDenseGated && INT8) y[i] *= __int2float_rn(static_cast<int>(u[4 * q + i])) * c1[i] * sa;
             if constexpr (EPI == kDenseGated && !INT8) y[i] *= __uint_as_float(u[4 * q + i]);
@@ -203,7 +220,7 @@ template <int CG, int OP, int EPI>
 __global__ void __launch_bounds__(608, 1)
 gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_constant__ CUtensorMap tm_a1,
                   const __grid_constant__ CUtensorMap tm_b0, const __grid_constant__ CUtensorMap tm_b1, const DenseParams p) {
-    using Cfg = DenseConfig<CG>;
+    using Cfg = DenseConfig;
     constexpr bool kInt8 = (OP == kOpInt8);
     constexpr bool kAMn = (OP == kOpBf16Tn);
     constexpr bool kBMn = (OP == kOpBf16Nn || OP == kOpBf16Tn);
@@ -292,43 +309,43 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
             const int end = min(i + p.kb_split, all_kb);
             int seg = (i >= p.num_kb) ? 1 : 0;
             for (int kb = i - seg * p.num_kb; i < end; ++i, ++kb) {
-                    if (kb == p.num_kb) { kb = 0; seg = 1; }
-                    const CUtensorMap* map = for_a ? ((second || seg) ? &tm_a1 : &tm_a0)
-                                                   : ((seg || (kGated && CG == 2 && rank)) ? &tm_b1 : &tm_b0);
-                    if (!mbar_wait(empty, phase ^ 1u)) {
-                        if (issuer) atomicCAS(p.status, 0, 101);
-                        ok = false;
-                        break;
-                    }
-                    if (issuer) {
-                        if (is_leader) mbar_arrive_expect_tx(full, CG * kbs * bytes);
-                        const uint32_t bar = full + peer;
+                if (kb == p.num_kb) { kb = 0; seg = 1; }
+                const CUtensorMap* map = for_a ? ((second || seg) ? &tm_a1 : &tm_a0)
+                                               : ((seg || (kGated && CG == 2 && rank)) ? &tm_b1 : &tm_b0);
+                if (!mbar_wait(empty, phase ^ 1u)) {
+                    if (issuer) atomicCAS(p.status, 0, 101);
+                    ok = false;
+                    break;
+                }
+                if (issuer) {
+                    if (is_leader) mbar_arrive_expect_tx(full, CG * kbs * bytes);
+                    const uint32_t bar = full + peer;
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            if (u == kbs) break;
-                            const int k = kb * kbs + u;             // past the end of K a load brings zeros
-                            const uint32_t to = dst + u * bytes;
-                            if (for_a) {
-                                if constexpr (kAMn) {
-                                    tma_load<CG>(to, map, bar, row_a * 2, k * 64, policy);
-                                    tma_load<CG>(to + 8192, map, bar, row_a * 2 + 128, k * 64, policy);
-                                } else {
-                                    tma_load<CG>(to, map, bar, k * 128, row_a, policy);
-                                }
-                            } else if constexpr (kBMn) {
-#pragma unroll
-                                for (int c = 0; c < 256 / CG; c += 64)
-                                    if (c < bn_cta) tma_load<CG>(to + c * 128, map, bar, (row_b + c) * 2, k * 64, policy);
+                    for (int u = 0; u < 2; ++u) {
+                        if (u == kbs) break;
+                        const int k = kb * kbs + u;             // past the end of K a load brings zeros
+                        const uint32_t to = dst + u * bytes;
+                        if (for_a) {
+                            if constexpr (kAMn) {
+                                tma_load<CG>(to, map, bar, row_a * 2, k * 64, policy);
+                                tma_load<CG>(to + 8192, map, bar, row_a * 2 + 128, k * 64, policy);
                             } else {
-                                tma_load<CG>(to, map, bar, k * 128, row_b, policy);
-                                if constexpr (kGated && CG == 1) tma_load<CG>(to + out_cols * 128, &tm_b1, bar, k * 128, row_b, policy);
+                                tma_load<CG>(to, map, bar, k * 128, row_a, policy);
                             }
+                        } else if constexpr (kBMn) {
+#pragma unroll
+                            for (int c = 0; c < 256 / CG; c += 64)
+                                if (c < bn_cta) tma_load<CG>(to + c * 128, map, bar, (row_b + c) * 2, k * 64, policy);
+                        } else {
+                            tma_load<CG>(to, map, bar, k * 128, row_b, policy);
+                            if constexpr (kGated && CG == 1) tma_load<CG>(to + out_cols * 128, &tm_b1, bar, k * 128, row_b, policy);
                         }
                     }
-                    dst += kbs * bytes;
-                    full += 8;
-                    empty += 8;
-                    if (full == bar_end) { dst = dst0; full = bar_full; empty = bar_empty; phase ^= 1u; }
+                }
+                dst += kbs * bytes;
+                full += 8;
+                empty += 8;
+                if (full == bar_end) { dst = dst0; full = bar_full; empty = bar_empty; phase ^= 1u; }
             }
         }
         // wait until every filled stage has been consumed: no copy or signal is outstanding when the CTA exits
@@ -455,51 +472,52 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
                         __syncwarp();
                     }
                 }
-            } else
-            for (int c0 = part * 32; c0 < out_cols; c0 += parts * 32) {
-                const int c1 = min(c0 + 32, out_cols);
-                for (int r = 0; r < results; ++r) {
-                    // 32 rows x up to 32 columns through a transpose in shared memory, so that a row's part of the result is
-                    // stored by neighbouring lanes
+            } else {
+                for (int c0 = part * 32; c0 < out_cols; c0 += parts * 32) {
+                    const int c1 = min(c0 + 32, out_cols);
+                    for (int r = 0; r < results; ++r) {
+                        // 32 rows x up to 32 columns through a transpose in shared memory, so that a row's part of the result is
+                        // stored by neighbouring lanes
 #pragma unroll 1
-                    for (int c = c0; c < c1; c += 16) {
-                        uint32_t v[16], u[16], w[8];
-                        tmem_ld_32x32b_x16(t_acc + c + ((kGated && r == 2) ? out_cols : 0), v);
-                        if (kGated && r == 0) tmem_ld_32x32b_x16(t_acc + out_cols + c, u);
-                        tmem_ld_wait();
-                        if (EPI == kDensePlain || r > 0) {
-                            dense_convert<false, kDensePlain, AVE_FP4_ACT_NONE>(v, v, w, sa, ColumnTerms<false, kDensePlain>{});
-                        } else {
-                            switch (p.act) {   // warp-uniform
-                                case AVE_FP4_ACT_RELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_RELU>(v, u, w, sa, terms); break;
-                                case AVE_FP4_ACT_GELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU>(v, u, w, sa, terms); break;
-                                case AVE_FP4_ACT_GELU_TANH: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU_TANH>(v, u, w, sa, terms); break;
-                                case AVE_FP4_ACT_SILU: dense_convert<kInt8, EPI, AVE_FP4_ACT_SILU>(v, u, w, sa, terms); break;
-                                default: dense_convert<kInt8, EPI, AVE_FP4_ACT_NONE>(v, u, w, sa, terms); break;
+                        for (int c = c0; c < c1; c += 16) {
+                            uint32_t v[16], u[16], w[8];
+                            tmem_ld_32x32b_x16(t_acc + c + ((kGated && r == 2) ? out_cols : 0), v);
+                            if (kGated && r == 0) tmem_ld_32x32b_x16(t_acc + out_cols + c, u);
+                            tmem_ld_wait();
+                            if (EPI == kDensePlain || r > 0) {
+                                dense_convert<false, kDensePlain, AVE_FP4_ACT_NONE>(v, v, w, sa, ColumnTerms<false, kDensePlain>{});
+                            } else {
+                                switch (p.act) {   // warp-uniform
+                                    case AVE_FP4_ACT_RELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_RELU>(v, u, w, sa, terms); break;
+                                    case AVE_FP4_ACT_GELU: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU>(v, u, w, sa, terms); break;
+                                    case AVE_FP4_ACT_GELU_TANH: dense_convert<kInt8, EPI, AVE_FP4_ACT_GELU_TANH>(v, u, w, sa, terms); break;
+                                    case AVE_FP4_ACT_SILU: dense_convert<kInt8, EPI, AVE_FP4_ACT_SILU>(v, u, w, sa, terms); break;
+                                    default: dense_convert<kInt8, EPI, AVE_FP4_ACT_NONE>(v, u, w, sa, terms); break;
+                                }
                             }
-                        }
-                        if constexpr (kInt8) {      // the next 16 columns' terms: in this group, or the first of the next one
-                            const int next = (c + 16 < c1) ? c + 16 : c0 + parts * 32;
-                            load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col0 + next, p.n);
-                        }
-                        const int q0 = (c - c0) / 8;
+                            if constexpr (kInt8) {      // the next 16 columns' terms: in this group, or the first of the next one
+                                const int next = (c + 16 < c1) ? c + 16 : c0 + parts * 32;
+                                load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col0 + next, p.n);
+                            }
+                            const int q0 = (c - c0) / 8;
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) stage_piece(sbuf, lane, q0 + q, w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-                    }
-                    __syncwarp();
-                    __nv_bfloat16* d = p.d[second ? 1 : 0];
-                    long long ld = p.ldd;
-                    if (kGated && r == 1) { d = p.gate; ld = p.ld_gate; }
-                    if (kGated && r == 2) { d = p.up; ld = p.ld_up; }
-                    const int c = c0 + (lane & 3) * 8;
-                    const bool col_ok = (c < c1) && (col0 + c < p.n);
+                            for (int q = 0; q < 2; ++q) stage_piece(sbuf, lane, q0 + q, w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+                        }
+                        __syncwarp();
+                        __nv_bfloat16* d = p.d[second ? 1 : 0];
+                        long long ld = p.ldd;
+                        if (kGated && r == 1) { d = p.gate; ld = p.ld_gate; }
+                        if (kGated && r == 2) { d = p.up; ld = p.ld_up; }
+                        const int c = c0 + (lane & 3) * 8;
+                        const bool col_ok = (c < c1) && (col0 + c < p.n);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int rr = i * 8 + (lane >> 2);
-                        const uint4 w = staged_piece(sbuf, rr, lane & 3);
-                        if (col_ok && row0 + rr < p.m) __stcs(reinterpret_cast<uint4*>(d + (row0 + rr) * ld + col0 + c), w);
+                        for (int i = 0; i < 4; ++i) {
+                            const int rr = i * 8 + (lane >> 2);
+                            const uint4 w = staged_piece(sbuf, rr, lane & 3);
+                            if (col_ok && row0 + rr < p.m) __stcs(reinterpret_cast<uint4*>(d + (row0 + rr) * ld + col0 + c), w);
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
             tcgen05_fence_before();
