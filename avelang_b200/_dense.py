@@ -28,6 +28,9 @@ def matrix(t: torch.Tensor, name: str, dtype: torch.dtype, rows: int | None = No
     if t.dim() != 2:
         raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}.")
     r, c = t.shape
+    if (t.is_contiguous() and not c & _ALIGNED[dtype] and not t.data_ptr() & 15 and (rows is None or r == rows)
+            and (cols is None or c == cols) and (t.is_cuda if device is None else t.device == device)):
+        return c
     if (rows is not None and r != rows) or (cols is not None and c != cols):
         raise ValueError(f"{name} must have shape {(r if rows is None else rows, c if cols is None else cols)}, got {(r, c)}.")
     if device is None:
@@ -69,6 +72,7 @@ def multiple(value: int, name: str, of: int, positive: bool = False) -> None:
 
 
 _functions: dict = {}
+_needs: dict = {}         # workspace sizes asked for last; they depend on the entry point, the device and the sizes alone
 MIN_CUT_BYTES = 4096      # AVE_DENSE_MIN_CUT_BYTES of include/ave_dense.h: shorter rows of K never need a workspace
 
 
@@ -105,9 +109,15 @@ def workspace(name: str, device: torch.device, *sizes) -> tuple[torch.Tensor | N
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return workspace(name, device, *sizes)
-    need = _function(name + "_workspace_bytes", dev)(*sizes)
-    if need < 0:
-        _lib.check(need)
+    key = (name, dev, sizes)
+    need = _needs.get(key)
+    if need is None:
+        need = _function(name + "_workspace_bytes", dev)(*sizes)
+        if need < 0:
+            _lib.check(need)
+        if len(_needs) >= 256:
+            _needs.clear()
+        _needs[key] = need
     if need == 0:
         return None, 0, 0
     t = torch.empty(need, dtype=torch.uint8, device=device)
