@@ -206,7 +206,12 @@ int launch_dense_cg(const HostDevice& dev, const DensePlan& plan, const Operand 
     p.num_kb = static_cast<int>(ceil_div(k * kElem, 128 * plan.kb_stage));
     p.tiles_m = static_cast<int>(ceil_div(m, 128 * CG));
     p.tiles_n = static_cast<int>(ceil_div(n, out_cols));
-    p.band = 8;
+    // Tile rows of a band: their A panels, some 32 MB, stay in L2 while the band goes through B.  Back to back under the power cap,
+    // bands of 8 / 16 rows: int8 8192^3 391 / 379 us, gated int8 4096 x 28672 x 8192 1288 / 1266, gated bf16 4096 x 16384 x 4096 840 /
+    // 814, 8192^3 1640 / 1698; the gradients of 8192 x 4096 x 16384 (operands as they lie in memory) 1627 / 1666.
+    p.band = kBMn ? 8 : static_cast<int>((int64_t(32) << 20) / (128 * CG * k * kElem));
+    if (p.band < 8) p.band = 8;
+    if (p.band > 16) p.band = 16;
     p.status = dev.status;
 
     CUtensorMap ta[2], tb[2];

@@ -38,7 +38,7 @@ def gemm_gated_transposed_b(x: torch.Tensor, W_gate: torch.Tensor, W_up: torch.T
 
     Sums, activation ("silu", "gelu", "gelu_tanh", "relu" or None) and product are fp32, rounded once.  ``save=True`` returns
     ``(out, gate, up)`` with the two products as bf16 (M, F), which gemm_gated_backward takes.  H and F must be multiples of 8,
-    M is free; up to 16 rows are served by a kernel that streams the weights.
+    M is free.  ``out`` may be a column block of a wider matrix; it may not overlap an operand.
     """
     act = _dense.activation_code(activation)
     ldx, ldg, ldu = _inputs(x, W_gate, W_up)

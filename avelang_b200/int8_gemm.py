@@ -93,8 +93,8 @@ def gemm_int8_transposed_b(A: Int8Operand, B: Int8Operand, out: torch.Tensor | N
     """``out = act(A @ B.T + bias)`` for integer operands A (M, K) and B (N, K), bf16 out.
 
     The integer sums are exact; scales, ``bias`` ((N,) bf16) and ``activation`` ("relu", "gelu", "gelu_tanh", "silu") are
-    applied in fp32 and the result is rounded once.  K must be a multiple of 16 up to 131056, N of 8, M is free; up to 16
-    rows are served by a kernel that streams the weights.
+    applied in fp32 and the result is rounded once.  K must be a multiple of 16 up to 131056, N of 8, M is free.  ``out`` may be a
+    column block of a wider matrix; it may not overlap an operand.
     """
     act = _dense.activation_code(activation)
     lda = _operand(A, "A")
@@ -119,7 +119,7 @@ def gemm_int8_gated_transposed_b(A: Int8Operand, W_gate: Int8Operand, W_up: Int8
                                  activation: str | None = "silu") -> torch.Tensor:
     """``out = act(A @ W_gate.T) * (A @ W_up.T)`` for integer operands A (M, K) and W_gate, W_up (F, K), bf16 out.
 
-    One kernel; both products stay on chip.  Limits as for gemm_int8_transposed_b (F a multiple of 8).
+    One pass; the two products never go through memory.  Limits as for gemm_int8_transposed_b (F a multiple of 8).
     """
     act = _dense.activation_code(activation)
     lda = _operand(A, "A")

@@ -317,3 +317,62 @@ def test_forward_with_long_sums(cuda_device, m, f, h):
             D.check(got, w, f"{activation} {what}")
         assert torch.equal(kept[0], ave.gemm_gated_transposed_b(x, wg, wu, activation=activation))
     ave.check_device_status(cuda_device)
+
+
+@pytest.mark.parametrize("m", [2, 20, 200])
+@pytest.mark.parametrize("activation", ACTS)
+def test_far_arguments_forward(cuda_device, m, activation):
+    """Gates over the whole range of bf16, through the streaming and the tile kernel: x is one-hot, so the gate is the weight itself."""
+    g = torch.cat([torch.linspace(-40, 40, 1001), torch.tensor([1e4, -1e4, 1e18, -1e18, 3e38, -3e38, 1e-30])]).to(torch.bfloat16)
+    f = g.numel() // 8 * 8
+    wg, wu = (torch.zeros((f, 16), dtype=torch.bfloat16, device=cuda_device) for _ in range(2))
+    wg[:, 3] = g[-f:].to(cuda_device)
+    wu[:, 3] = 1.0
+    x = torch.zeros((m, 16), dtype=torch.bfloat16, device=cuda_device)
+    x[:, 3] = 1.0
+    gd = wg[:, 3].double().expand(m, f)
+    want = D.act(gd, activation)
+    if activation == "gelu_tanh":
+        want = torch.where(gd > 1e10, gd, torch.where(gd < -1e10, torch.zeros_like(gd), want))      # the cube overflows in the plain form
+    got = ave.gemm_gated_transposed_b(x, wg, wu, activation=activation)
+    D.check(got, (want, D.BF16 * want.abs() + 1e-37))
+
+
+def test_gradients_beyond_two_to_the_31_elements(cuda_device):
+    m, f, h = 66000, 32776, 8
+    g = torch.Generator(device=cuda_device).manual_seed(0)
+    dout, gate, up = (torch.randn((m, f), generator=g, device=cuda_device, dtype=torch.bfloat16) for _ in range(3))
+    x, wg, wu = _randn(cuda_device, m, h, 4), _randn(cuda_device, f, h, 5), _randn(cuda_device, f, h, 6)
+    dx, dwg, dwu = ave.gemm_gated_backward(dout, x, wg, wu, gate, up)
+    ave.check_device_status(cuda_device)
+    for rows in (slice(0, 2), slice(32767, 32770), slice(65534, 65538), slice(m - 2, m)):
+        want = D.gated_backward(dout[rows], x[rows], wg, wu, gate[rows], up[rows], "silu")
+        D.check(dx[rows], want[0], f"{rows}")
+    for cols in (slice(0, 8), slice(16384, 16392), slice(f - 8, f)):
+        want = D.gated_backward(dout[:, cols], x, wg[cols], wu[cols], gate[:, cols], up[:, cols], "silu")
+        D.check(dwg[cols], want[1], f"{cols}")
+        D.check(dwu[cols], want[2], f"{cols}")
+
+
+@pytest.mark.parametrize("m,n,k", [(64, 72, 4104), (777, 1032, 4104), (300, 5000, 136), (2000, 264, 520)])
+def test_operands_overwritten_right_after_a_call(cuda_device, m, n, k):
+    """The second product of a backward pass starts before the first has ended: whatever is queued next still finds both done."""
+    a, b, dout = _randn(cuda_device, m, k, 1), _randn(cuda_device, n, k, 2), _randn(cuda_device, m, n, 3)
+    wg, wu, gate, up = b.clone(), b.clone(), _randn(cuda_device, m, n, 4), _randn(cuda_device, m, n, 5)
+    da, db = ave.gemm_transposed_b_backward(dout, a, b)
+    dx, dwg, dwu = ave.gemm_gated_backward(dout, a, wg, wu, gate, up)
+    got = []
+    for _ in range(20):
+        got.append(ave.gemm_transposed_b_backward(dout, a, b))
+        a.neg_()
+        b.neg_()
+        got.append(ave.gemm_gated_backward(dout, a, wg, wu, gate, up))
+        dout.neg_()
+        wg.neg_()
+        wu.neg_()
+    for i in range(20):
+        # before iteration i all five have changed sign i times, and x once more before its second call
+        assert torch.equal(got[2 * i][0], da) and torch.equal(got[2 * i][1], db)      # two changed signs each
+        assert torch.equal(got[2 * i + 1][0], dx)                                    # dout and the weights
+        assert torch.equal(got[2 * i + 1][1], -dwg) and torch.equal(got[2 * i + 1][2], -dwu)      # dout and x
+    ave.check_device_status(cuda_device)

@@ -118,6 +118,16 @@ def test_int8_sums_are_exact(cuda_device, m):
     assert torch.equal(ave.gemm_int8_transposed_b(a, b), want)
 
 
+@pytest.mark.parametrize("m,n,k", [(40, 64, 8208), (890, 264, 8208), (12, 2504, 4112)])
+def test_int8_sums_are_exact_when_cut(cuda_device, m, n, k):
+    a, b = _ints(cuda_device, m, k, 1), _ints(cuda_device, n, k, 2)
+    a.scales.fill_(1.0)
+    b.scales.fill_(1.0)
+    want = a.values.double() @ b.values.double().T
+    assert want.abs().max() < 2 ** 24
+    assert torch.equal(ave.gemm_int8_transposed_b(a, b), want.float().to(torch.bfloat16))
+
+
 @pytest.mark.parametrize("m", [4, 24, 150])
 @pytest.mark.parametrize("low", [-127, -128])
 def test_int8_largest_sums(cuda_device, m, low):
@@ -285,3 +295,36 @@ def test_two_host_threads_on_streams_of_their_own(cuda_device):
         t.join()
     assert not bad
     ave.check_device_status(cuda_device)
+
+
+@pytest.mark.parametrize("m", [3, 30, 300])
+@pytest.mark.parametrize("activation", ACTS)
+def test_far_arguments(cuda_device, m, activation):
+    """Arguments of the activation over a wide range, from the scales: codes of 1 and -1, scales up to 1e30."""
+    n = 1008
+    a = ave.Int8Operand(torch.zeros((m, 32), dtype=torch.int8, device=cuda_device), torch.ones(m, device=cuda_device))
+    a.values[:, 5] = 1
+    b = ave.Int8Operand(torch.zeros((n, 32), dtype=torch.int8, device=cuda_device), torch.logspace(-20, 30, n, device=cuda_device))
+    b.values[::2, 5] = 1
+    b.values[1::2, 5] = -1
+    want, bound = D.int8_gemm(a, b, None, activation)
+    if activation == "gelu_tanh":
+        z = a.values[:, 5:6].double() * b.values[:, 5].double() * b.scales.double()
+        want = torch.where(z > 1e10, z, torch.where(z < -1e10, torch.zeros_like(z), want))      # the cube overflows in the plain form
+        bound = D.BF16 * want.abs() + 1.13 * 4 * 2.0 ** -24 * z.abs()
+    D.check(ave.gemm_int8_transposed_b(a, b, activation=activation), (want, bound))
+
+
+@pytest.mark.parametrize("m", [1, 12, 60, 300])
+def test_one_operand_overwritten_again_and_again(cuda_device, m):
+    """Each kernel is launched under the previous one's tail: the product sees the codes and scales of its own step."""
+    k, n = 1040, 520
+    xs = [_randn(cuda_device, m, k, s, 10.0 ** (s % 7 - 3)) for s in range(14)]
+    w = _ints(cuda_device, n, k, 99)
+    want = [ave.gemm_int8_transposed_b(ave.quantize_int8(x), w) for x in xs]
+    torch.cuda.synchronize()
+    q = ave.quantize_int8(xs[0])
+    for _ in range(10):
+        got = [ave.gemm_int8_transposed_b(ave.quantize_int8(x, out=q), w) for x in xs]
+        for g, e in zip(got, want):
+            assert torch.equal(g, e)
