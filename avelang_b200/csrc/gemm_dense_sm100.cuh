@@ -23,13 +23,13 @@
 // columns, and block_n is a run-time value: the number of columns goes into the instruction descriptor, so the host picks
 // it, and cuts of K for long sums of few tiles, by an estimate of the launch's clocks (plan_dense in ave_dense_api.cu).
 //
-// Measured on a B200, one launch, operands not in L2 (burst; back to back the power cap takes some 15 %): int8 8192^3 327 us
-// (3.36 POP/s, twice the rate of cuBLAS in bf16), gated int8 4096 x 28672 x 8192 1.09 ms (3.53 POP/s), gated bf16 4096 x 16384 x
-// 4096 665 us (1.65 PFLOP/s), C = A B and C = A^T B of 8192 x 4096 x 16384 0.70 and 0.69 ms (1.57 PFLOP/s): bound by the tensor
-// pipe.  int8 16 x 28672 x 8192 42.5 us (5.5 TB/s) and gated bf16 128 x 14336 x 8192 82 us (5.7 TB/s): bound by reading the weights.
-// With a K block of less than 256 columns the operands' way from L2 is the limit (50 to 64 bytes a clock and SM), and below
-// some 10 us the launch is: 0.8 us until the first operands are there, 0.3 until the first accumulator, 0.5 to 1 for the epilogue
-// and 0.3 to 0.7 to leave.
+// Measured on a B200, operands not in L2 (burst; back to back the power cap takes some 15 %): int8 8192^3 327 us (3.36 POP/s,
+// twice the rate of cuBLAS in bf16), gated int8 4096 x 28672 x 8192 1.09 ms (3.53 POP/s), gated bf16 4096 x 16384 x 4096 665 us
+// (1.65 PFLOP/s), both gradients of 8192 x 4096 x 16384 1.34 ms (1.64 PFLOP/s): bound by the tensor pipe.  int8 16 x 28672 x 8192
+// 41 us (5.7 TB/s) and gated bf16 128 x 14336 x 8192 82 us (5.7 TB/s): bound by reading the weights.  In tiles narrower than 256
+// columns the operands' way from L2 is the limit (50 to 85 bytes a clock and SM, less the more SMs ask), and below some 10 us the
+// launch is: 0.8 us until the first operands are there, 0.3 until the first accumulator, 0.5 to 1 for the epilogue and 0.3 to 0.7
+// to leave.
 //
 // An MN-major operand tile is kept as boxes of 64 elements (one swizzled 128-byte row) x 64 K rows, 8 KB each: the
 // matrix descriptor steps 8 KB from one box to the next along MN (leading offset) and 1 KB from one group of eight
