@@ -68,6 +68,8 @@ struct DenseParams {
     int act;
     int wait_late;                   // the previous kernel in the stream writes nothing that this one reads or writes: run beside
                                      // its tail and wait for it (so that whoever waits for this one has waited for both) at the end
+    int early, early_items;          // of a wait_late launch: its first `early` clusters start that many tiles ahead of the others, on
+                                     // SMs that the previous kernel has left, and take so many tiles before the rest is dealt out
     int trigger_late;                // let the next kernel start only once the previous one has finished (the next is wait_late)
     __nv_bfloat16* gate;             // gated: where to keep G and U, or nullptr
     __nv_bfloat16* up;
@@ -280,6 +282,14 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     tcgen05_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_gen, 0);
 
+    // The i-th work item of this cluster, or one past the last
+    const int dealt = p.early * p.early_items;
+    auto item = [&](int i) {
+        if (cluster_id >= p.early) return dealt + cluster_id - p.early + i * num_clusters;
+        if (i < p.early_items) return cluster_id + i * p.early;
+        return dealt + num_clusters - p.early + cluster_id + (i - p.early_items) * num_clusters;
+    };
+
     // Operands may come from the previous kernel.  All roles wait for it here, so that none of the bounded waits below counts its time.
     if (threadIdx.x == 0 && !p.trigger_late) pdl_launch_dependents();
     if (!p.wait_late) pdl_wait_prior_grid();
@@ -299,7 +309,7 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
         uint32_t dst = dst0, full = bar_full, empty = bar_empty;
         uint32_t phase = 0;
         bool ok = true;
-        for (int t = cluster_id; t < num_tiles && ok; t += num_clusters) {
+        for (int n_item = 0, t = item(0); t < num_tiles && ok; t = item(++n_item)) {
             int tm, tn, split;
             dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn, split);
             const bool second = tm >= p.tiles_m;                  // tile of the second result
@@ -371,7 +381,7 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
             uint32_t phase = 0;
             int tile_iter = 0;
             bool ok = true;
-            for (int t = cluster_id; t < num_tiles && ok; t += num_clusters, ++tile_iter) {
+            for (int t = item(0); t < num_tiles && ok; t = item(++tile_iter)) {
                 const int acc = tile_iter & 1;
                 const uint32_t acc_phase = static_cast<uint32_t>(tile_iter >> 1) & 1u;
                 if (!mbar_wait(bar_tempty + acc * 8, acc_phase ^ 1u)) {
@@ -430,7 +440,7 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
         const uint32_t tempty0 = (CG == 2) ? mapa_shared(bar_tempty, 0) : bar_tempty;
         const int results = (kGated && p.gate != nullptr) ? 3 : 1;
         int tile_iter = 0;
-        for (int t = cluster_id; t < num_tiles; t += num_clusters, ++tile_iter) {
+        for (int t = item(0); t < num_tiles; t = item(++tile_iter)) {
             int tm, tn, split;
             dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn, split);
             const bool second = tm >= p.tiles_m;
