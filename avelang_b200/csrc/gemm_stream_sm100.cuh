@@ -5,8 +5,8 @@
 // One persistent CTA per SM owns an even share of the weight rows, in groups of 8, over the whole of K: nothing is exchanged
 // between CTAs, so there is no workspace, no counter, and the sums have the same order on every call.  A producer warp copies
 // units of 16 rows, 4 KB of K per row and stage, into two shared-memory stages of 64 KB with plain bulk copies (no tensor
-// map: a row's piece is contiguous), which keeps 128 KB in flight per SM; a third stage where the activations leave room in L1.  Sixteen warps split each stage's K, 256 bytes of
-// every row each, and add up in shared memory at the end of a unit.
+// map: a row's piece is contiguous), which keeps 128 KB in flight per SM; a third stage where the activations leave room in L1.
+// Sixteen warps split each stage's K, 256 bytes of every row each, and add up in shared memory at the end of a unit.
 //
 // What the shape was chosen by (one token, us): int8 28672 x 8192 59 with units of 32 rows, 1 KB pieces and 8 warps, 50 with
 // 16 rows and 2 KB, 40 with 16 warps, 39 with 4 KB pieces (floor 35.8); gated int8 2 x 28672 x 8192 110, 79, 73 and 71 (floor
@@ -200,7 +200,6 @@ gemm_stream_kernel(const StreamParams p) {
                 ok = false;
             }
             const uint8_t* tile = smem + stage * kStreamStageBytes + g * kStreamRowStride + k_mine;
-            
             const int at = k * kStreamSpan + k_mine;
 #pragma unroll
             for (int s = 0; s < kPieces; ++s) {

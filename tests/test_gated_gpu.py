@@ -376,3 +376,31 @@ def test_operands_overwritten_right_after_a_call(cuda_device, m, n, k):
         assert torch.equal(got[2 * i + 1][0], dx)                                    # dout and the weights
         assert torch.equal(got[2 * i + 1][1], -dwg) and torch.equal(got[2 * i + 1][2], -dwu)      # dout and x
     ave.check_device_status(cuda_device)
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 2552, 2048), (16, 120, 40008), (300, 128, 40008), (264, 2216, 2784), (777, 1032, 4104)])
+def test_second_product_ahead_of_the_first_ones_end(cuda_device, m, n, k):
+    # the first product's last wave leaves SMs to the second's first clusters, in all four mixes of pairs and single CTAs
+    a, b, dout = _randn(cuda_device, m, k, 1), _randn(cuda_device, n, k, 2, k ** -0.5), _randn(cuda_device, m, n, 3, 0.1)
+    want = D.product_backward(dout, a, b)
+    da = ave.gemm_transposed_b_backward(dout, a, b, need_db=False)[0]
+    db = ave.gemm_transposed_b_backward(dout, a, b, need_da=False)[1]
+    for _ in range(3):
+        got = ave.gemm_transposed_b_backward(dout, a, b)
+        for g, w, alone, what in zip(got, want, (da, db), ("da", "db")):
+            D.check(g, w, what)
+            assert torch.equal(g, alone)
+    ave.check_device_status(cuda_device)
+
+
+@pytest.mark.parametrize("m,f,h", [(8, 2824, 1664), (16, 1664, 1704), (32, 2672, 2736), (520, 1200, 2000)])
+def test_second_product_ahead_gated(cuda_device, m, f, h):
+    x, wg, wu = _randn(cuda_device, m, h, 1), _randn(cuda_device, f, h, 2, h ** -0.5), _randn(cuda_device, f, h, 3, h ** -0.5)
+    dout, gate, up = (_randn(cuda_device, m, f, s) for s in (4, 5, 6))
+    got = ave.gemm_gated_backward(dout, x, wg, wu, gate, up)
+    for g, w, what in zip(got, D.gated_backward(dout, x, wg, wu, gate, up, "silu"), ("dx", "dw_gate", "dw_up")):
+        D.check(g, w, what)
+    assert torch.equal(got[0], ave.gemm_gated_backward(dout, x, wg, wu, gate, up, need_dw=False)[0])
+    alone = ave.gemm_gated_backward(dout, x, wg, wu, gate, up, need_dx=False)
+    assert torch.equal(got[1], alone[1]) and torch.equal(got[2], alone[2])
+    ave.check_device_status(cuda_device)
