@@ -248,18 +248,23 @@ int launch_dense(const HostDevice& dev, const DensePlan& plan, const Operand (&a
 
 // The second product of a backward pass starts on the SMs that the first one's last wave leaves out, one of the first one's items
 // ahead of the rest.  How many tiles those clusters take before the rest is dealt out to all: what ends the launch soonest.
-// Without and with, us: product_backward 777x1032x4104 24.5 and 22.8, 365x5624x13008 129 and 116; gated_backward 2443x7408x2832
-// 334 and 320; unchanged where the first product's last wave is full (2048x4096x1024: 68.3) or the items are as many either way.
+// A tile of the second product takes its products' time or, with a short sum, its share of writing the result: 2100 bytes a clock,
+// 4.1 TB/s (without the latter 64x8192x8192 went from 62 to 92 us).
+// Without and with, in turn, us: product_backward 777x1032x4104 24.7 and 22.9, 365x5624x13008 126 and 117, 1303x13360x3376 264
+// and 196; gated_backward 2443x7408x2832 386 and 364; unchanged where the first product's last wave is full (2048x4096x1024: 74).
+// Over 130 backward passes of sizes spread at random, 1 % on average, 25 % at most.
 void deal_early(const HostDevice& dev, const DensePlan& first, const DensePlan& second, DenseParams& p) {
     const int64_t clusters = dev.sm_count / first.cg, grid = dev.sm_count / second.cg;
     const int64_t rest = first.items % clusters;
     const int64_t early = rest == 0 ? 0 : (clusters - rest) * first.cg / second.cg;
     if (early == 0 || early >= grid || second.items <= grid) return;
+    const int64_t write = 128 * second.block_n * (second.splits > 1 ? 4 : 2) * int64_t(dev.sm_count) / 2100;
+    const int64_t clk = second.clk > write ? second.clk : write;
     int64_t best = INT64_MAX;
-    for (int64_t ahead = 0; ahead <= first.clk / second.clk + 1 && ahead * early < second.items; ++ahead) {
+    for (int64_t ahead = 0; ahead <= first.clk / clk + 1 && ahead * early < second.items; ++ahead) {
         const int64_t left = second.items - ahead * early, rounds = left / grid, more = left % grid;
-        const int64_t late_end = first.clk + (rounds + (more > 0 ? 1 : 0)) * second.clk;
-        const int64_t early_end = (ahead + rounds + (more > grid - early ? 1 : 0)) * second.clk;
+        const int64_t late_end = first.clk + (rounds + (more > 0 ? 1 : 0)) * clk;
+        const int64_t early_end = (ahead + rounds + (more > grid - early ? 1 : 0)) * clk;
         const int64_t end = late_end > early_end ? late_end : early_end;
         if (end < best) {
             best = end;

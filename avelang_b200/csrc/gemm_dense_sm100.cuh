@@ -282,13 +282,11 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
     tcgen05_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_ptr_gen, 0);
 
-    // The i-th work item of this cluster, or one past the last
-    const int dealt = p.early * p.early_items;
-    auto item = [&](int i) {
-        if (cluster_id >= p.early) return dealt + cluster_id - p.early + i * num_clusters;
-        if (i < p.early_items) return cluster_id + i * p.early;
-        return dealt + num_clusters - p.early + cluster_id + (i - p.early_items) * num_clusters;
-    };
+    // This cluster's first work item, and the step from its i-th one to the next: the early clusters share out the first items among
+    // themselves, then all of them take turns.
+    const int ahead = cluster_id < p.early ? p.early_items : 0;
+    const int first_item = cluster_id < p.early ? cluster_id : cluster_id + (p.early_items - 1) * p.early;
+    auto step = [&](int i) { return i + 1 < ahead ? p.early : num_clusters; };
 
     // Operands may come from the previous kernel.  All roles wait for it here, so that none of the bounded waits below counts its time.
     if (threadIdx.x == 0 && !p.trigger_late) pdl_launch_dependents();
@@ -309,16 +307,16 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
         uint32_t dst = dst0, full = bar_full, empty = bar_empty;
         uint32_t phase = 0;
         bool ok = true;
-        for (int n_item = 0, t = item(0); t < num_tiles && ok; t = item(++n_item)) {
+        for (int i = 0, t = first_item; t < num_tiles && ok; t += step(i++)) {
             int tm, tn, split;
             dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn, split);
             const bool second = tm >= p.tiles_m;                  // tile of the second result
             const int row_a = ((second ? tm - p.tiles_m : tm) * CG + rank) * 128;
             const int row_b = tn * out_cols + (kGated ? 0 : rank * bn_cta);
-            int i = split * p.kb_split;
-            const int end = min(i + p.kb_split, all_kb);
-            int seg = (i >= p.num_kb) ? 1 : 0;
-            for (int kb = i - seg * p.num_kb; i < end; ++i, ++kb) {
+            int at = split * p.kb_split;
+            const int end = min(at + p.kb_split, all_kb);
+            int seg = (at >= p.num_kb) ? 1 : 0;
+            for (int kb = at - seg * p.num_kb; at < end; ++at, ++kb) {
                 if (kb == p.num_kb) { kb = 0; seg = 1; }
                 const CUtensorMap* map = for_a ? ((second || seg) ? &tm_a1 : &tm_a0)
                                                : ((seg || (kGated && CG == 2 && rank)) ? &tm_b1 : &tm_b0);
@@ -381,7 +379,7 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
             uint32_t phase = 0;
             int tile_iter = 0;
             bool ok = true;
-            for (int t = item(0); t < num_tiles && ok; t = item(++tile_iter)) {
+            for (int t = first_item; t < num_tiles && ok; t += step(tile_iter++)) {
                 const int acc = tile_iter & 1;
                 const uint32_t acc_phase = static_cast<uint32_t>(tile_iter >> 1) & 1u;
                 if (!mbar_wait(bar_tempty + acc * 8, acc_phase ^ 1u)) {
@@ -440,7 +438,7 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
         const uint32_t tempty0 = (CG == 2) ? mapa_shared(bar_tempty, 0) : bar_tempty;
         const int results = (kGated && p.gate != nullptr) ? 3 : 1;
         int tile_iter = 0;
-        for (int t = item(0); t < num_tiles; t = item(++tile_iter)) {
+        for (int t = first_item; t < num_tiles; t += step(tile_iter++)) {
             int tm, tn, split;
             dense_tile(t, tile_rows, p.tiles_n, p.band, tm, tn, split);
             const bool second = tm >= p.tiles_m;
