@@ -104,6 +104,8 @@ struct DensePlan {
     int a_rows, b_rows, kb_stage, stages;
     int64_t items;   // tiles times ranges
     int64_t clk;     // estimate of one
+    int64_t sums;    // estimate of writing and reading the ranges' sums
+    int early, early_items;      // of the second product of a backward pass: see DenseParams
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -116,10 +118,13 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // left out), at most 40 of them for one SM.  Work comes in waves of all CTAs.  Cutting K into S ranges costs writing and reading S fp32
 // results (2600 bytes a clock) and a launch.  Against sweeps of widths and cuts at 27 sizes the choice was within 14 % of
 // the best one, within 5 % for most.
-DensePlan plan_dense(int sms, int64_t m, int64_t cols, int64_t k_bytes, int segments, int batches, bool a_mn, bool b_mn,
-                     bool gated, bool may_split) {
-    DensePlan best{};
-    int64_t best_cost = INT64_MAX;
+//
+// each_plan calls f(plan) for every tile width, CTA pairs or not and number of ranges.
+constexpr int64_t kSumsLaunch = 5500;
+
+template <class F>
+void each_plan(int sms, int64_t m, int64_t cols, int64_t k_bytes, int segments, int batches, bool a_mn, bool b_mn, bool gated, bool may_split,
+               F f) {
     for (int cg = (m <= 128 ? 1 : 2); cg >= 1; --cg) {
         const int64_t clusters = sms / cg;
         const int64_t tile_rows = ceil_div(m, 128 * cg) * batches;
@@ -144,17 +149,28 @@ DensePlan plan_dense(int sms, int64_t m, int64_t cols, int64_t k_bytes, int segm
                 if (splits > 1 && tiles * (splits - 1) >= clusters) break;       // a wave is full without more of them
                 const int64_t kb_split = ceil_div(steps, splits);
                 const int64_t ranges = ceil_div(steps, kb_split);
-                int64_t cost = ceil_div(tiles * ranges, clusters) * (kb_split * kbs * clk + 400);
-                if (ranges > 1) cost += ranges * m * batches * cols * 8 / 2600 + 5500;
-                if (cost < best_cost) {
-                    best_cost = cost;
-                    best = DensePlan{cg, bn, static_cast<int>(ranges), static_cast<int>(kb_split), a_rows, b_rows, kbs, 0, tiles * ranges,
-                                     kb_split * kbs * clk + 400};
-                }
+                f(DensePlan{cg, bn, static_cast<int>(ranges), static_cast<int>(kb_split), a_rows, b_rows, kbs,
+                            DenseConfig::stages(a_rows, b_rows, kbs), tiles * ranges, kb_split * kbs * clk + 400,
+                            ranges > 1 ? ranges * m * batches * cols * 8 / 2600 : 0, 0, 0});
             }
         }
     }
-    best.stages = DenseConfig::stages(best.a_rows, best.b_rows, best.kb_stage);
+}
+
+int64_t launch_clocks(int sms, const DensePlan& p) {
+    return ceil_div(p.items, sms / p.cg) * p.clk + (p.splits > 1 ? p.sums + kSumsLaunch : 0);
+}
+
+DensePlan plan_dense(int sms, int64_t m, int64_t cols, int64_t k_bytes, bool gated, bool may_split) {
+    DensePlan best{};
+    int64_t best_cost = INT64_MAX;
+    each_plan(sms, m, cols, k_bytes, 1, 1, false, false, gated, may_split, [&](const DensePlan& p) {
+        const int64_t cost = launch_clocks(sms, p);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = p;
+        }
+    });
     return best;
 }
 
@@ -164,28 +180,31 @@ constexpr int64_t elem_bytes() { return OP == kOpInt8 ? 1 : 2; }
 // Forward products cut K only from here on: below they ask for no workspace, and a caller need not ask.
 bool forward_may_cut(int64_t m, int64_t k_bytes) { return m > 8 && k_bytes >= AVE_DENSE_MIN_CUT_BYTES; }
 
-// m, n: sizes of one result; k: sum length of one segment.  A plan depends on the sizes alone and takes as long to find as a
-// small product runs, a few microseconds: each host thread keeps the last ones it made.
+// A plan depends on the sizes alone and takes as long to find as a small product runs, a few microseconds: each host thread keeps the
+// last ones it made, in slots by a hash of the sizes.
+constexpr int kPlanSlots = 64;
+
+int plan_slot(int64_t m, int64_t n, int64_t k) {
+    const uint64_t h = (static_cast<uint64_t>(m) * 0x9E3779B97F4A7C15ull) ^ (static_cast<uint64_t>(n) * 0xC2B2AE3D27D4EB4Full) ^ static_cast<uint64_t>(k);
+    return static_cast<int>(((h * 0xD6E8FEB86659FD93ull) >> 32) % kPlanSlots);
+}
+
+// A forward product's plan.
 template <int OP, int EPI>
-DensePlan plan_for(const HostDevice& dev, int64_t m, int64_t n, int64_t k, int segments, int batches) {
+DensePlan plan_for(const HostDevice& dev, int64_t m, int64_t n, int64_t k) {
     struct Slot {
         int64_t m, n, k;
-        int sms, segments, batches;
+        int sms;
         DensePlan plan;
     };
-    constexpr int kSlots = 64;
-    thread_local Slot slots[kSlots] = {};
-    uint64_t h = (static_cast<uint64_t>(m) * 0x9E3779B97F4A7C15ull) ^ (static_cast<uint64_t>(n) * 0xC2B2AE3D27D4EB4Full) ^ static_cast<uint64_t>(k);
-    Slot& slot = slots[((h * 0xD6E8FEB86659FD93ull) >> 32) % kSlots];
-    if (slot.m != m || slot.n != n || slot.k != k || slot.sms != dev.sm_count || slot.segments != segments || slot.batches != batches) {
-        slot.plan = plan_dense(dev.sm_count, m, EPI == kDenseGated ? 2 * n : n, k * elem_bytes<OP>(), segments, batches, OP == kOpBf16Tn,
-                               OP == kOpBf16Nn || OP == kOpBf16Tn, EPI == kDenseGated, EPI == kDensePlain || forward_may_cut(m, k * elem_bytes<OP>()));
+    thread_local Slot slots[kPlanSlots] = {};
+    Slot& slot = slots[plan_slot(m, n, k)];
+    if (slot.m != m || slot.n != n || slot.k != k || slot.sms != dev.sm_count) {
+        slot.plan = plan_dense(dev.sm_count, m, EPI == kDenseGated ? 2 * n : n, k * elem_bytes<OP>(), EPI == kDenseGated, forward_may_cut(m, k * elem_bytes<OP>()));
         slot.m = m;
         slot.n = n;
         slot.k = k;
         slot.sms = dev.sm_count;
-        slot.segments = segments;
-        slot.batches = batches;
     }
     return slot.plan;
 }
@@ -246,32 +265,139 @@ int launch_dense(const HostDevice& dev, const DensePlan& plan, const Operand (&a
     return launch_dense_cg<2, OP, EPI>(dev, plan, a, b, m, n, k, p, stream);
 }
 
-// The second product of a backward pass starts on the SMs that the first one's last wave leaves out, one of the first one's items
-// ahead of the rest.  How many tiles those clusters take before the rest is dealt out to all: what ends the launch soonest.
+// Two products in a row, the second of which needs nothing of the first (DenseParams::wait_late): it starts on the SMs that the
+// first one's last wave leaves out, one of the first one's items ahead of the rest.  How many tiles those clusters take before the
+// rest is dealt out to all: what ends the launch soonest.
 // A tile of the second product takes its products' time or, with a short sum, its share of writing the result: 2100 bytes a clock,
 // 4.1 TB/s (without the latter 64x8192x8192 went from 62 to 92 us).
-// Without and with, in turn, us: product_backward 777x1032x4104 24.7 and 22.9, 365x5624x13008 126 and 117, 1303x13360x3376 264
-// and 196; gated_backward 2443x7408x2832 386 and 364; unchanged where the first product's last wave is full (2048x4096x1024: 74).
-// Over 130 backward passes of sizes spread at random, 1 % on average, 25 % at most.
-void deal_early(const HostDevice& dev, const DensePlan& first, const DensePlan& second, DenseParams& p) {
-    const int64_t clusters = dev.sm_count / first.cg, grid = dev.sm_count / second.cg;
+// Returns the clocks from the start of the first one's last wave on.
+int64_t deal_early(int sms, const DensePlan& first, DensePlan& second) {
+    const int64_t clusters = sms / first.cg, grid = sms / second.cg;
     const int64_t rest = first.items % clusters;
     const int64_t early = rest == 0 ? 0 : (clusters - rest) * first.cg / second.cg;
-    if (early == 0 || early >= grid || second.items <= grid) return;
-    const int64_t write = 128 * second.block_n * (second.splits > 1 ? 4 : 2) * int64_t(dev.sm_count) / 2100;
+    const int64_t active = second.items < grid ? second.items : grid;
+    const int64_t write = int64_t(128) * second.cg * second.block_n * (second.splits > 1 ? 4 : 2) * active / 2100;
     const int64_t clk = second.clk > write ? second.clk : write;
-    int64_t best = INT64_MAX;
-    for (int64_t ahead = 0; ahead <= first.clk / clk + 1 && ahead * early < second.items; ++ahead) {
+    second.early = second.early_items = 0;
+    if (second.items <= early) return first.clk > clk ? first.clk : clk;
+    int64_t best = first.clk + ceil_div(second.items, grid) * clk;
+    if (early == 0 || early >= grid || second.items <= grid) return best;
+    for (int64_t ahead = 1; ahead <= first.clk / clk + 1 && ahead * early < second.items; ++ahead) {
         const int64_t left = second.items - ahead * early, rounds = left / grid, more = left % grid;
         const int64_t late_end = first.clk + (rounds + (more > 0 ? 1 : 0)) * clk;
         const int64_t early_end = (ahead + rounds + (more > grid - early ? 1 : 0)) * clk;
         const int64_t end = late_end > early_end ? late_end : early_end;
         if (end < best) {
             best = end;
-            p.early_items = static_cast<int>(ahead);
+            second.early_items = static_cast<int>(ahead);
+            second.early = static_cast<int>(early);
         }
     }
-    p.early = p.early_items > 0 ? static_cast<int>(early) : 0;
+    return best;
+}
+
+// Plans of two such products, found together: what the first leaves idle the second fills, so a cut of the first one's K that would
+// pay for it alone often does not.  And plans of each alone, with the same ranges of K: a gradient's bits do not depend on
+// whether the other is asked for.
+struct PairPlan {
+    DensePlan first, second, first_alone, second_alone;
+};
+
+// Choices for one of them: for every number of ranges, the ones that take the least time alone.
+struct PlanChoices {
+    static constexpr int kEach = 4;
+    DensePlan plan[8][kEach];
+    int64_t cost[8][kEach];
+    int count[8] = {};
+
+    void add(int sms, const DensePlan& p) {
+        const int64_t c = launch_clocks(sms, p);
+        DensePlan(&plans)[kEach] = plan[p.splits - 1];
+        int64_t(&costs)[kEach] = cost[p.splits - 1];
+        int& n = count[p.splits - 1];
+        if (n == kEach && c >= costs[kEach - 1]) return;
+        int at = n < kEach ? n++ : kEach - 1;
+        for (; at > 0 && costs[at - 1] > c; --at) {
+            costs[at] = costs[at - 1];
+            plans[at] = plans[at - 1];
+        }
+        costs[at] = c;
+        plans[at] = p;
+    }
+    template <class F>
+    void each(F f) const {
+        for (int s = 0; s < 8; ++s)
+            for (int i = 0; i < count[s]; ++i) f(plan[s][i]);
+    }
+};
+
+// Both products in turn, each planned alone / both together, us: gated backward 1003x2744x1048 41.5 / 36.9, 1144x1040x216 21.6 / 17.7,
+// product gradients 744x7384x248 21.5 / 16.0, 6480x584x216 19.8 / 13.7; the worst of 220 sizes 880x1800x160 11.1 / 12.3, on average
+// 1.7 % less.  Left as planned alone: what memory bounds for half of the time or more (8x11504x2264 31 / 43, for all SMs share that
+// however the tiles lie), and what would gain less than 5 % by the estimate (2048x4096x1024 69 / 73).
+//
+// C0 = A B with m0 x n0 results over `segments` sums of length k0, and C1 = A^T B with `batches` results of m1 x n1 and sums of length k1
+PairPlan plan_pair(int sms, int64_t m0, int64_t n0, int64_t k0, int segments, int64_t m1, int64_t n1, int64_t k1, int batches) {
+    PlanChoices a, b;
+    each_plan(sms, m0, n0, 2 * k0, segments, 1, false, true, false, true, [&](const DensePlan& p) { a.add(sms, p); });
+    each_plan(sms, m1, n1, 2 * k1, 1, batches, true, true, false, true, [&](const DensePlan& p) { b.add(sms, p); });
+    auto least = [&](const PlanChoices& of) {
+        DensePlan p{};
+        of.each([&](const DensePlan& c) { if (p.cg == 0 || launch_clocks(sms, c) < launch_clocks(sms, p)) p = c; });
+        return p;
+    };
+    auto together = [&](const DensePlan& first, DensePlan& second) {
+        return (ceil_div(first.items, sms / first.cg) - 1) * first.clk + first.sums + deal_early(sms, first, second) + second.sums +
+               (first.splits > 1 || second.splits > 1 ? kSumsLaunch : 0);
+    };
+    PairPlan best{least(a), least(b), {}, {}};
+    const int64_t memory = 2 * segments * k0 * (m0 + n0) / 3300 + 2 * (m0 * n0 + batches * m1 * n1) / 2100;
+    const bool by_memory = 2 * memory > launch_clocks(sms, best.first) + launch_clocks(sms, best.second);
+    int64_t best_cost = together(best.first, best.second) * 19 / 20;
+    if (!by_memory) a.each([&](const DensePlan& first) {
+        b.each([&](const DensePlan& choice) {
+            DensePlan second = choice;
+            const int64_t cost = together(first, second);
+            if (cost < best_cost) {
+                best_cost = cost;
+                best.first = first;
+                best.second = second;
+            }
+        });
+    });
+    auto alone = [&](const PlanChoices& of, const DensePlan& like) {
+        DensePlan p{};
+        of.each([&](const DensePlan& c) {
+            if (c.splits != like.splits || (c.splits > 1 && (c.kb_stage != like.kb_stage || c.kb_split != like.kb_split))) return;
+            if (p.cg == 0 || launch_clocks(sms, c) < launch_clocks(sms, p)) p = c;
+        });
+        return p;
+    };
+    best.first_alone = alone(a, best.first);
+    best.second_alone = alone(b, best.second);
+    return best;
+}
+
+// As plan_for: found once for a size and kept by each host thread.
+const PairPlan& pair_for(const HostDevice& dev, int64_t m, int64_t n, int64_t k, bool gated) {
+    struct Slot {
+        int64_t m, n, k;
+        int sms;
+        bool gated;
+        PairPlan plan;
+    };
+    thread_local Slot slots[kPlanSlots] = {};
+    Slot& slot = slots[plan_slot(m, n, k)];
+    if (slot.m != m || slot.n != n || slot.k != k || slot.sms != dev.sm_count || slot.gated != gated) {
+        // gated: dX (m, k) = dG Wg + dU Wu over n, dWg and dWu (n, k) over m; else dA (m, k) over n and dB (n, k) over m
+        slot.plan = plan_pair(dev.sm_count, m, k, n, gated ? 2 : 1, n, k, m, gated ? 2 : 1);
+        slot.m = m;
+        slot.n = n;
+        slot.k = k;
+        slot.sms = dev.sm_count;
+        slot.gated = gated;
+    }
+    return slot.plan;
 }
 
 int64_t split_words(const DensePlan& plan, int64_t rows, int64_t n) { return plan.splits > 1 ? plan.splits * rows * n : 0; }
@@ -306,7 +432,7 @@ bool stream_rows(const HostDevice& dev, int64_t m, int64_t weight_rows, int64_t 
 template <int OP, int EPI>
 int launch_forward(const HostDevice& dev, const char* fn, const Operand (&a)[2], const Operand (&b)[2], int64_t m, int64_t n, int64_t k,
                    DenseParams p, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
-    const DensePlan plan = plan_for<OP, EPI>(dev, m, n, k, 1, 1);
+    const DensePlan plan = plan_for<OP, EPI>(dev, m, n, k);
     int rc = check_workspace(fn, workspace, workspace_bytes, 4 * split_words(plan, m, EPI == kDenseGated ? 2 * n : n));
     if (rc) return rc;
     p.partial = static_cast<uint32_t*>(workspace);
@@ -331,7 +457,7 @@ int64_t forward_workspace(const char* fn, int64_t m, int64_t n, int64_t k) {
     if (rc) return rc < 0 ? rc : -rc;
     const int64_t cols = EPI == kDenseGated ? 2 * n : n;
     if (!forward_may_cut(m, k * elem_bytes<OP>()) || stream_rows(dev, m, cols, k * elem_bytes<OP>())) return 0;
-    return 4 * split_words(plan_for<OP, EPI>(dev, m, n, k, 1, 1), m, cols);
+    return 4 * split_words(plan_for<OP, EPI>(dev, m, n, k), m, cols);
 }
 
 DenseParams dense_params() {
@@ -655,14 +781,11 @@ GatedBackwardPlan plan_gated_backward(const HostDevice& dev, int64_t m, int64_t 
     GatedBackwardPlan p{};
     p.ld = ceil_div(f, 64) * 64;
     p.half = ceil_div(m * p.ld * 2, 256) * 256;
-    if (want_x) {
-        p.dx = plan_for<kOpBf16Nn, kDensePlain>(dev, m, h, f, 2, 1);
-        p.dx_words = split_words(p.dx, m, h);
-    }
-    if (want_w) {
-        p.dw = plan_for<kOpBf16Tn, kDensePlain>(dev, f, h, m, 1, 2);
-        p.dw_words = split_words(p.dw, 2 * f, h);
-    }
+    const PairPlan& pair = pair_for(dev, m, f, h, true);
+    p.dx = want_w ? pair.first : pair.first_alone;
+    p.dw = want_x ? pair.second : pair.second_alone;
+    if (want_x) p.dx_words = split_words(p.dx, m, h);
+    if (want_w) p.dw_words = split_words(p.dw, 2 * f, h);
     return p;
 }
 
@@ -674,14 +797,11 @@ struct ProductBackwardPlan {
 
 ProductBackwardPlan plan_product_backward(const HostDevice& dev, int64_t m, int64_t n, int64_t k, bool want_a, bool want_b) {
     ProductBackwardPlan p{};
-    if (want_a) {
-        p.da = plan_for<kOpBf16Nn, kDensePlain>(dev, m, k, n, 1, 1);
-        p.da_words = split_words(p.da, m, k);
-    }
-    if (want_b) {
-        p.db = plan_for<kOpBf16Tn, kDensePlain>(dev, n, k, m, 1, 1);
-        p.db_words = split_words(p.db, n, k);
-    }
+    const PairPlan& pair = pair_for(dev, m, n, k, false);
+    p.da = want_b ? pair.first : pair.first_alone;
+    p.db = want_a ? pair.second : pair.second_alone;
+    if (want_a) p.da_words = split_words(p.da, m, k);
+    if (want_b) p.db_words = split_words(p.db, n, k);
     return p;
 }
 
@@ -771,7 +891,8 @@ int ave_bf16_gated_backward(const void* dd, int64_t ld_dd, const void* x, int64_
         p.ldd = row_stride(f, h, ld_dw);
         p.partial = dw_partial;
         p.wait_late = want_x;
-        if (want_x) deal_early(dev, plan.dx, plan.dw, p);
+        p.early = plan.dw.early;
+        p.early_items = plan.dw.early_items;
         CHECK((launch_dense<kOpBf16Tn, kDensePlain>(dev, plan.dw, {{d_gate, ld}, {d_up, ld}}, {{x, ldx}, {x, ldx}}, f, h, m, p, s)));
         sums.job[1] = split_sum(plan.dw, dw_partial, 2 * f * h, dw_gate, p.ldd, f, h);
         sums.job[2] = split_sum(plan.dw, dw_partial + f * h, 2 * f * h, dw_up, p.ldd, f, h);
@@ -831,7 +952,8 @@ int ave_bf16_gemm_backward(const void* dd, int64_t ld_dd, const void* a, int64_t
         p.ldd = row_stride(n, k, ld_db);
         p.partial = db_partial;
         p.wait_late = da != nullptr;
-        if (da != nullptr) deal_early(dev, plan.da, plan.db, p);
+        p.early = plan.db.early;
+        p.early_items = plan.db.early_items;
         CHECK((launch_dense<kOpBf16Tn, kDensePlain>(dev, plan.db, {{dd, ld_dd}, {dd, ld_dd}}, {{a, lda}, {a, lda}}, n, k, m, p, s)));
         sums.job[1] = split_sum(plan.db, db_partial, n * k, db, p.ldd, n, k);
     }
