@@ -105,6 +105,7 @@ struct DensePlan {
     int64_t items;   // tiles times ranges
     int64_t clk;     // estimate of one
     int64_t sums;    // estimate of writing and reading the ranges' sums
+    int sms;         // SMs it runs on
     int early, early_items;      // of the second product of a backward pass: see DenseParams
 };
 
@@ -151,21 +152,21 @@ void each_plan(int sms, int64_t m, int64_t cols, int64_t k_bytes, int segments, 
                 const int64_t ranges = ceil_div(steps, kb_split);
                 f(DensePlan{cg, bn, static_cast<int>(ranges), static_cast<int>(kb_split), a_rows, b_rows, kbs,
                             DenseConfig::stages(a_rows, b_rows, kbs), tiles * ranges, kb_split * kbs * clk + 400,
-                            ranges > 1 ? ranges * m * batches * cols * 8 / 2600 : 0, 0, 0});
+                            ranges > 1 ? ranges * m * batches * cols * 8 / 2600 : 0, sms, 0, 0});
             }
         }
     }
 }
 
-int64_t launch_clocks(int sms, const DensePlan& p) {
-    return ceil_div(p.items, sms / p.cg) * p.clk + (p.splits > 1 ? p.sums + kSumsLaunch : 0);
+int64_t launch_clocks(const DensePlan& p) {
+    return ceil_div(p.items, p.sms / p.cg) * p.clk + (p.splits > 1 ? p.sums + kSumsLaunch : 0);
 }
 
 DensePlan plan_dense(int sms, int64_t m, int64_t cols, int64_t k_bytes, bool gated, bool may_split) {
     DensePlan best{};
     int64_t best_cost = INT64_MAX;
     each_plan(sms, m, cols, k_bytes, 1, 1, false, false, gated, may_split, [&](const DensePlan& p) {
-        const int64_t cost = launch_clocks(sms, p);
+        const int64_t cost = launch_clocks(p);
         if (cost < best_cost) {
             best_cost = cost;
             best = p;
@@ -248,7 +249,7 @@ int launch_dense_cg(const HostDevice& dev, const DensePlan& plan, const Operand 
         if (rc) return rc;
     }
     const int64_t items = int64_t(p.tiles_m) * p.batches * p.tiles_n * p.splits;
-    const int64_t clusters = dev.sm_count / CG;
+    const int64_t clusters = plan.sms / CG;
     // 16 epilogue warps hide more latency (int8 8192 x 8192 x 1024 78 -> 63 us), 8 start sooner (64 x 64 x 64 3.6 against 4.0 us):
     // tiles of up to 64 result columns keep two warps of a quadrant busy and no more, and the plain epilogue is short.
     const int threads = Cfg::threads(EPI != kDensePlain && out_cols > 64 ? 16 : 8);
@@ -310,8 +311,8 @@ struct PlanChoices {
     int64_t cost[8][kEach];
     int count[8] = {};
 
-    void add(int sms, const DensePlan& p) {
-        const int64_t c = launch_clocks(sms, p);
+    void add(const DensePlan& p) {
+        const int64_t c = launch_clocks(p);
         DensePlan(&plans)[kEach] = plan[p.splits - 1];
         int64_t(&costs)[kEach] = cost[p.splits - 1];
         int& n = count[p.splits - 1];
@@ -335,46 +336,53 @@ struct PlanChoices {
 // product gradients 744x7384x248 21.5 / 16.0, 6480x584x216 19.8 / 13.7; the worst of 220 sizes 880x1800x160 11.1 / 12.3, on average
 // 1.7 % less.  Left as planned alone: what memory bounds for half of the time or more (8x11504x2264 31 / 43, for all SMs share that
 // however the tiles lie), and what would gain less than 5 % by the estimate (2048x4096x1024 69 / 73).
+// Where memory bounds the products of a few rows, one of which reads the weights and the other writes their gradients, they run
+// beside each other, each on half of the SMs: copying goes at 6.2 TB/s, writing alone at 4.  The second's CTAs are single ones, for
+// pairs find no two free neighbours, and take 85 % of its tiles before the first is done.  One after the other / beside each other,
+// us: product gradients 64x8192x8192 61 / 54, 64x4096x4096 25.9 / 19.9, 32x20064x4048 72.5 / 67; gated backward 16x14336x4096 104 / 93,
+// 64x4096x4096 38.6 / 36.4; with two tile rows, 256x8192x8192 73.9 / 75.1, not.
 //
 // C0 = A B with m0 x n0 results over `segments` sums of length k0, and C1 = A^T B with `batches` results of m1 x n1 and sums of length k1
 PairPlan plan_pair(int sms, int64_t m0, int64_t n0, int64_t k0, int segments, int64_t m1, int64_t n1, int64_t k1, int batches) {
-    PlanChoices a, b;
-    each_plan(sms, m0, n0, 2 * k0, segments, 1, false, true, false, true, [&](const DensePlan& p) { a.add(sms, p); });
-    each_plan(sms, m1, n1, 2 * k1, 1, batches, true, true, false, true, [&](const DensePlan& p) { b.add(sms, p); });
-    auto least = [&](const PlanChoices& of) {
-        DensePlan p{};
-        of.each([&](const DensePlan& c) { if (p.cg == 0 || launch_clocks(sms, c) < launch_clocks(sms, p)) p = c; });
-        return p;
-    };
+    auto each_first = [&](int on, auto f) { each_plan(on, m0, n0, 2 * k0, segments, 1, false, true, false, true, f); };
+    auto each_second = [&](auto f) { each_plan(sms, m1, n1, 2 * k1, 1, batches, true, true, false, true, f); };
+    auto take = [](DensePlan& least, const DensePlan& p) { if (least.cg == 0 || launch_clocks(p) < launch_clocks(least)) least = p; };
     auto together = [&](const DensePlan& first, DensePlan& second) {
         return (ceil_div(first.items, sms / first.cg) - 1) * first.clk + first.sums + deal_early(sms, first, second) + second.sums +
                (first.splits > 1 || second.splits > 1 ? kSumsLaunch : 0);
     };
-    PairPlan best{least(a), least(b), {}, {}};
+    PairPlan best{};
+    PlanChoices a, b;
+    each_first(sms, [&](const DensePlan& p) { a.add(p); take(best.first, p); });
+    each_second([&](const DensePlan& p) { b.add(p); take(best.second, p); });
     const int64_t memory = 2 * segments * k0 * (m0 + n0) / 3300 + 2 * (m0 * n0 + batches * m1 * n1) / 2100;
-    const bool by_memory = 2 * memory > launch_clocks(sms, best.first) + launch_clocks(sms, best.second);
-    int64_t best_cost = together(best.first, best.second) * 19 / 20;
-    if (!by_memory) a.each([&](const DensePlan& first) {
-        b.each([&](const DensePlan& choice) {
-            DensePlan second = choice;
-            const int64_t cost = together(first, second);
-            if (cost < best_cost) {
-                best_cost = cost;
-                best.first = first;
-                best.second = second;
-            }
+    const bool by_memory = 2 * memory > launch_clocks(best.first) + launch_clocks(best.second);
+    if (by_memory && m0 <= 128) {
+        const int half = sms / 2;
+        best = PairPlan{};
+        each_first(half, [&](const DensePlan& p) { take(best.first, p); });
+        each_second([&](const DensePlan& p) { if (p.cg == 1) take(best.second, p); });
+        best.second.early_items = static_cast<int>(best.second.items * 85 / 100 / (sms - half));
+        best.second.early = best.second.early_items > 0 ? sms - half : 0;
+    } else {
+        int64_t best_cost = together(best.first, best.second) * 19 / 20;
+        if (!by_memory) a.each([&](const DensePlan& first) {
+            b.each([&](const DensePlan& choice) {
+                DensePlan second = choice;
+                const int64_t cost = together(first, second);
+                if (cost < best_cost) {
+                    best_cost = cost;
+                    best.first = first;
+                    best.second = second;
+                }
+            });
         });
-    });
-    auto alone = [&](const PlanChoices& of, const DensePlan& like) {
-        DensePlan p{};
-        of.each([&](const DensePlan& c) {
-            if (c.splits != like.splits || (c.splits > 1 && (c.kb_stage != like.kb_stage || c.kb_split != like.kb_split))) return;
-            if (p.cg == 0 || launch_clocks(sms, c) < launch_clocks(sms, p)) p = c;
-        });
-        return p;
+    }
+    auto same_ranges = [](const DensePlan& p, const DensePlan& q) {
+        return p.splits == q.splits && (p.splits == 1 || (p.kb_stage == q.kb_stage && p.kb_split == q.kb_split));
     };
-    best.first_alone = alone(a, best.first);
-    best.second_alone = alone(b, best.second);
+    each_first(sms, [&](const DensePlan& p) { if (same_ranges(p, best.first)) take(best.first_alone, p); });
+    each_second([&](const DensePlan& p) { if (same_ranges(p, best.second)) take(best.second_alone, p); });
     return best;
 }
 

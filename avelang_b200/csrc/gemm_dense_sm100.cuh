@@ -68,8 +68,8 @@ struct DenseParams {
     int act;
     int wait_late;                   // the previous kernel in the stream writes nothing that this one reads or writes: run beside
                                      // its tail and wait for it (so that whoever waits for this one has waited for both) at the end
-    int early, early_items;          // of a wait_late launch: its first `early` clusters start that many tiles ahead of the others, on
-                                     // SMs that the previous kernel has left, and take so many tiles before the rest is dealt out
+    int early, early_items;          // of a wait_late launch: its first `early` clusters start ahead of the others, on SMs that the
+                                     // previous kernel has left or not used, and take so many tiles each before the rest is dealt out
     int trigger_late;                // let the next kernel start only once the previous one has finished (the next is wait_late)
     __nv_bfloat16* gate;             // gated: where to keep G and U, or nullptr
     __nv_bfloat16* up;

@@ -379,7 +379,8 @@ def test_operands_overwritten_right_after_a_call(cuda_device, m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(8, 2552, 2048), (16, 120, 40008), (300, 128, 40008), (264, 2216, 2784), (777, 1032, 4104),
-                                   (753, 2912, 288), (744, 7384, 248), (880, 1800, 160), (393, 3104, 448), (1024, 4096, 1024)])
+                                   (753, 2912, 288), (744, 7384, 248), (880, 1800, 160), (393, 3104, 448), (1024, 4096, 1024),
+                                   (64, 4096, 4096), (1, 2048, 4104), (128, 8200, 1032)])
 def test_second_product_ahead_of_the_first_ones_end(cuda_device, m, n, k):
     # the first product's last wave leaves SMs to the second's first clusters, in all four mixes of pairs and single CTAs
     a, b, dout = _randn(cuda_device, m, k, 1), _randn(cuda_device, n, k, 2, k ** -0.5), _randn(cuda_device, m, n, 3, 0.1)
@@ -395,7 +396,7 @@ def test_second_product_ahead_of_the_first_ones_end(cuda_device, m, n, k):
 
 
 @pytest.mark.parametrize("m,f,h", [(8, 2824, 1664), (16, 1664, 1704), (32, 2672, 2736), (520, 1200, 2000), (1003, 2744, 1048), (424, 1488, 528),
-                                   (1144, 1040, 216), (8, 80, 120), (1760, 1376, 488)])
+                                   (1144, 1040, 216), (8, 80, 120), (1760, 1376, 488), (24, 5432, 2632), (1, 8200, 520), (128, 4096, 2048)])
 def test_second_product_ahead_gated(cuda_device, m, f, h):
     x, wg, wu = _randn(cuda_device, m, h, 1), _randn(cuda_device, f, h, 2, h ** -0.5), _randn(cuda_device, f, h, 3, h ** -0.5)
     dout, gate, up = (_randn(cuda_device, m, f, s) for s in (4, 5, 6))
