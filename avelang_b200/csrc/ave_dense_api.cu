@@ -235,6 +235,7 @@ int launch_dense_cg(const HostDevice& dev, const DensePlan& plan, const Operand 
     p.band = kBMn ? 8 : static_cast<int>((int64_t(32) << 20) / (128 * CG * k * kElem));
     if (p.band < 8) p.band = 8;
     if (p.band > 16) p.band = 16;
+    p.direct = EPI == kDenseScaled && out_cols % 16 == 0 && p.ldd % 16 == 0 && (reinterpret_cast<uintptr_t>(p.d[0]) & 31u) == 0;
     p.status = dev.status;
 
     CUtensorMap ta[2], tb[2];

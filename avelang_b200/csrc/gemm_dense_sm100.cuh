@@ -70,6 +70,7 @@ struct DenseParams {
                                      // its tail and wait for it (so that whoever waits for this one has waited for both) at the end
     int early, early_items;          // of a wait_late launch: its first `early` clusters start ahead of the others, on SMs that the
                                      // previous kernel has left or not used, and take so many tiles each before the rest is dealt out
+    int direct;                      // scaled: rows and tiles of D lie on 32 bytes, a thread stores its row's 16 columns as it has them
     int trigger_late;                // let the next kernel start only once the previous one has finished (the next is wait_late)
     __nv_bfloat16* gate;             // gated: where to keep G and U, or nullptr
     __nv_bfloat16* up;
@@ -202,6 +203,13 @@ __device__ __forceinline__ void dense_convert(const uint32_t (&v)[16], const uin
         w[2 * q] = pack_bf16(y[0], y[1]);
         w[2 * q + 1] = pack_bf16(y[2], y[3]);
     }
+}
+
+// 16 columns of a row, on 32 bytes
+__device__ __forceinline__ void store_16(__nv_bfloat16* at, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
 }
 
 // A warp's 2 KB transpose buffer: 64 bytes per row, 16-byte piece q of row r in place q ^ (r / 2 & 3), so that eight lanes
@@ -485,7 +493,11 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
                     const int c1 = min(c0 + 32, out_cols);
                     for (int r = 0; r < results; ++r) {
                         // 32 rows x up to 32 columns through a transpose in shared memory, so that a row's part of the result is
-                        // stored by neighbouring lanes
+                        // stored by neighbouring lanes.  Or directly, in whole 32-byte sectors: at the tensor pipe's full rate its
+                        // operands take all of shared memory's 128 bytes a clock, and the transpose slows it down.  int8 with gelu_tanh and
+                        // bias, transposed / direct, us: 2048 x 8192 x 1024 37.2 / 35.0, 8192 x 8192 x 512 76 / 71, 8192^3 the same; gated
+                        // int8 4096 x 8192 x 1024 56.5 / 55.8, gated bf16 4096 x 16384 x 4096 805 / 808, and gradients of 512 x 8192 x 8192,
+                        // bound by writing, 110 / 117, so the others keep to the transpose.
 #pragma unroll 1
                         for (int c = c0; c < c1; c += 16) {
                             uint32_t v[16], u[16], w[8];
@@ -507,10 +519,22 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
                                 const int next = (c + 16 < c1) ? c + 16 : c0 + parts * 32;
                                 load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col0 + next, p.n);
                             }
+                            if constexpr (EPI == kDenseScaled) {
+                                if (p.direct) {
+                                    const int col = col0 + c;
+                                    __nv_bfloat16* at = p.d[0] + (row0 + lane) * p.ldd + col;
+                                    if (row0 + lane < p.m) {
+                                        if (col + 16 <= p.n) store_16(at, w);
+                                        else if (col < p.n) *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+                                    }
+                                    continue;
+                                }
+                            }
                             const int q0 = (c - c0) / 8;
 #pragma unroll
                             for (int q = 0; q < 2; ++q) stage_piece(sbuf, lane, q0 + q, w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
                         }
+                        if (EPI == kDenseScaled && p.direct) continue;
                         __syncwarp();
                         __nv_bfloat16* d = p.d[second ? 1 : 0];
                         long long ld = p.ldd;

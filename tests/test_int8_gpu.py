@@ -328,3 +328,19 @@ def test_one_operand_overwritten_again_and_again(cuda_device, m):
         got = [ave.gemm_int8_transposed_b(ave.quantize_int8(x, out=q), w) for x in xs]
         for g, e in zip(got, want):
             assert torch.equal(g, e)
+
+
+@pytest.mark.parametrize("m,n,k", [(20, 520, 128), (130, 1000, 64), (300, 2056, 272), (257, 4096, 1024)])
+def test_results_on_and_off_32_bytes(cuda_device, m, n, k):
+    # rows that lie on 32 bytes are stored in another way than rows on 16: same bits, and nothing beside them is touched
+    a, b, bias = _ints(cuda_device, m, k, 1, 1.0), _ints(cuda_device, n, k, 2, 1.0), _randn(cuda_device, 1, n, 3)[0]
+    want = ave.gemm_int8_transposed_b(a, b, bias=bias, activation="gelu")
+    wide = (n + 15) // 16 * 16
+    for width, first in ((wide + 32, 16), (wide + 32, 8), (wide + 40, 16), (wide + 40, 24)):
+        hold = torch.full((m + 2, width), 7.0, dtype=torch.bfloat16, device=cuda_device)
+        out = hold[1:m + 1, first:first + n]
+        assert ave.gemm_int8_transposed_b(a, b, out=out, bias=bias, activation="gelu") is out
+        assert torch.equal(out, want)
+        out.fill_(7.0)
+        assert (hold == 7.0).all()
+    ave.check_device_status(cuda_device)
