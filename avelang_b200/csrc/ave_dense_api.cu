@@ -341,13 +341,20 @@ struct PlanChoices {
 // beside each other, each on half of the SMs: copying goes at 6.2 TB/s, writing alone at 4.  The second's CTAs are single ones, for
 // pairs find no two free neighbours, and take 85 % of its tiles before the first is done.  One after the other / beside each other,
 // us: product gradients 64x8192x8192 61 / 54, 64x4096x4096 25.9 / 19.9, 32x20064x4048 72.5 / 67; gated backward 16x14336x4096 104 / 93,
-// 64x4096x4096 38.6 / 36.4; with two tile rows, 256x8192x8192 73.9 / 75.1, not.
+// 64x4096x4096 38.6 / 36.4; with two tile rows, 256x8192x8192 73.9 / 75.1, not.  Ranges that suit half of the SMs and cost the product
+// far more when it is asked for alone (32x20064x4048 30 / 47) give way to those it would have alone.
 //
 // C0 = A B with m0 x n0 results over `segments` sums of length k0, and C1 = A^T B with `batches` results of m1 x n1 and sums of length k1
 PairPlan plan_pair(int sms, int64_t m0, int64_t n0, int64_t k0, int segments, int64_t m1, int64_t n1, int64_t k1, int batches) {
     auto each_first = [&](int on, auto f) { each_plan(on, m0, n0, 2 * k0, segments, 1, false, true, false, true, f); };
     auto each_second = [&](auto f) { each_plan(sms, m1, n1, 2 * k1, 1, batches, true, true, false, true, f); };
     auto take = [](DensePlan& least, const DensePlan& p) { if (least.cg == 0 || launch_clocks(p) < launch_clocks(least)) least = p; };
+    // (a segment of an odd number of K blocks ends inside a stage of two)
+    const bool odd = segments == 2 && ceil_div(k0, 64) % 2 != 0;
+    auto same_ranges = [odd](const DensePlan& p, const DensePlan& q) {
+        if (odd && p.splits > 1 && p.kb_stage != q.kb_stage) return false;
+        return p.splits == q.splits && (p.splits == 1 || p.kb_stage * p.kb_split == q.kb_stage * q.kb_split);
+    };
     auto together = [&](const DensePlan& first, DensePlan& second) {
         return (ceil_div(first.items, sms / first.cg) - 1) * first.clk + first.sums + deal_early(sms, first, second) + second.sums +
                (first.splits > 1 || second.splits > 1 ? kSumsLaunch : 0);
@@ -360,8 +367,17 @@ PairPlan plan_pair(int sms, int64_t m0, int64_t n0, int64_t k0, int segments, in
     const bool by_memory = 2 * memory > launch_clocks(best.first) + launch_clocks(best.second);
     if (by_memory && m0 <= 128) {
         const int half = sms / 2;
-        best = PairPlan{};
+        const DensePlan whole = best.first;
+        DensePlan alone{};
+        best.first = DensePlan{};
         each_first(half, [&](const DensePlan& p) { take(best.first, p); });
+        each_first(sms, [&](const DensePlan& p) { if (same_ranges(p, best.first)) take(alone, p); });
+        if (launch_clocks(alone) * 10 > launch_clocks(whole) * 13) {      // ranges that would cost it too much alone
+            best.first = whole;
+            best.first.sms = half;
+            each_first(half, [&](const DensePlan& p) { if (same_ranges(p, whole)) take(best.first, p); });
+        }
+        best.second = DensePlan{};
         each_second([&](const DensePlan& p) { if (p.cg == 1) take(best.second, p); });
         best.second.early_items = static_cast<int>(best.second.items * 85 / 100 / (sms - half));
         best.second.early = best.second.early_items > 0 ? sms - half : 0;
@@ -379,9 +395,6 @@ PairPlan plan_pair(int sms, int64_t m0, int64_t n0, int64_t k0, int segments, in
             });
         });
     }
-    auto same_ranges = [](const DensePlan& p, const DensePlan& q) {
-        return p.splits == q.splits && (p.splits == 1 || (p.kb_stage == q.kb_stage && p.kb_split == q.kb_split));
-    };
     each_first(sms, [&](const DensePlan& p) { if (same_ranges(p, best.first)) take(best.first_alone, p); });
     each_second([&](const DensePlan& p) { if (same_ranges(p, best.second)) take(best.second_alone, p); });
     return best;
