@@ -25,18 +25,17 @@ __device__ __forceinline__ void gated_backward_pair(uint32_t d, uint32_t g, uint
 // One 16-byte piece (8 columns) of each matrix per thread and step; f8 = F / 8.
 template <int ACT>
 __global__ void __launch_bounds__(256)
-gated_backward_kernel(const __nv_bfloat16* __restrict__ dout, long long ld_dout, const __nv_bfloat16* __restrict__ gate, long long ld_gate,
-                      const __nv_bfloat16* __restrict__ up, long long ld_up, __nv_bfloat16* __restrict__ d_gate,
-                      __nv_bfloat16* __restrict__ d_up, long long ld, long long rows, int f8) {
+gated_backward_kernel(const __nv_bfloat16* dout, long long ld_dout, const __nv_bfloat16* gate, long long ld_gate, const __nv_bfloat16* up,
+                      long long ld_up, __nv_bfloat16* d_gate, __nv_bfloat16* d_up, long long ld, long long rows, int f8) {
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const long long total = rows * f8;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
         const long long r = i / f8;
         const long long c = (i - r * f8) * 8;
-        const uint4 d = __ldcs(reinterpret_cast<const uint4*>(dout + r * ld_dout + c));
-        const uint4 g = __ldcs(reinterpret_cast<const uint4*>(gate + r * ld_gate + c));
-        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(up + r * ld_up + c));
+        const uint4 d = load_16<true>(dout + r * ld_dout + c);
+        const uint4 g = load_16<true>(gate + r * ld_gate + c);
+        const uint4 u = load_16<true>(up + r * ld_up + c);
         uint4 dg, du;
         gated_backward_pair<ACT>(d.x, g.x, u.x, dg.x, du.x);
         gated_backward_pair<ACT>(d.y, g.y, u.y, dg.y, du.y);

@@ -164,14 +164,14 @@ __device__ __forceinline__ void load_terms(ColumnTerms<INT8, EPI>& t, const floa
     for (int h = 0; h < 2; ++h) {
         const int at = min(col + 8 * h, n - 8);
         if constexpr (INT8) {
-            t.s0[2 * h] = __ldg(reinterpret_cast<const float4*>(sb0 + at));
-            t.s0[2 * h + 1] = __ldg(reinterpret_cast<const float4*>(sb0 + at) + 1);
+            t.s0[2 * h] = load_f32x4(sb0 + at);
+            t.s0[2 * h + 1] = load_f32x4(sb0 + at + 4);
             if constexpr (EPI == kDenseGated) {
-                t.s1[2 * h] = __ldg(reinterpret_cast<const float4*>(sb1 + at));
-                t.s1[2 * h + 1] = __ldg(reinterpret_cast<const float4*>(sb1 + at) + 1);
+                t.s1[2 * h] = load_f32x4(sb1 + at);
+                t.s1[2 * h + 1] = load_f32x4(sb1 + at + 4);
             }
         }
-        if constexpr (EPI == kDenseScaled) t.bias[h] = (bias != nullptr) ? __ldg(reinterpret_cast<const uint4*>(bias + at)) : make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (EPI == kDenseScaled) t.bias[h] = (bias != nullptr) ? load_16(bias + at) : make_uint4(0u, 0u, 0u, 0u);
     }
 }
 
@@ -456,7 +456,7 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
             const int col0 = tn * out_cols;
             float sa = 1.0f;
             // the row's scale and the first columns' scales and bias come while the products still run
-            if constexpr (kInt8) sa = (row0 + lane < p.m) ? __ldg(p.a_scale + row0 + lane) : 0.0f;
+            if constexpr (kInt8) sa = (row0 + lane < p.m) ? load_f32(p.a_scale + row0 + lane) : 0.0f;
             ColumnTerms<kInt8, EPI> terms;
             load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col0 + part * 32, p.n);
             if (!mbar_wait(bar_tfull + acc * 8, acc_phase)) {
@@ -585,7 +585,7 @@ struct SplitSums {
 // 8 columns of a K range added to the sums so far
 template <bool INT8>
 __device__ __forceinline__ void add_range(uint32_t (&acc)[8], const uint32_t* src) {
-    const uint4 lo = __ldcs(reinterpret_cast<const uint4*>(src)), hi = __ldcs(reinterpret_cast<const uint4*>(src) + 1);
+    const uint4 lo = load_16<true>(src), hi = load_16<true>(src + 4);
     const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -633,7 +633,7 @@ finish_splits_kernel(const DenseParams p) {
             add_range<INT8>(g, src);
             if constexpr (EPI == kDenseGated) add_range<INT8>(u, src + slab);
         }
-        const float sa = INT8 ? __ldg(p.a_scale + row) : 1.0f;
+        const float sa = INT8 ? load_f32(p.a_scale + row) : 1.0f;
         ColumnTerms<INT8, EPI> terms;
         load_terms(terms, p.b_scale[0], p.b_scale[1], p.bias, col, p.n);
         uint32_t v16[16], u16[16], w[8];

@@ -175,8 +175,8 @@ gemm_stream_kernel(const StreamParams p) {
         for (int s = 0; s < kPieces; ++s) {
             const int at = k * kStreamSpan + s * 64;
             const bool in = at + k_mine < p.k_bytes;   // k_bytes % 16 == 0
-            a[s] = (in && lo) ? __ldg(reinterpret_cast<const uint4*>(xlo + at)) : zero;
-            if constexpr (!M8) b[s] = (in && hi) ? __ldg(reinterpret_cast<const uint4*>(xhi + at)) : zero;
+            a[s] = load_16(xlo + at, in && lo);
+            if constexpr (!M8) b[s] = load_16(xhi + at, in && hi);
             else b[s] = zero;
         }
     };
@@ -252,12 +252,12 @@ gemm_stream_kernel(const StreamParams p) {
             float y = total(c);
             float sx = 1.0f;
             if constexpr (INT8) {
-                sx = __ldg(p.x_scale + m);
-                y = y * __ldg(p.w_scale[0] + n) * sx;
+                sx = load_f32(p.x_scale + m);
+                y = y * load_f32(p.w_scale[0] + n) * sx;
             }
             if constexpr (GATED) {
                 float u = total(cols + c);
-                if constexpr (INT8) u = u * __ldg(p.w_scale[1] + n) * sx;
+                if constexpr (INT8) u = u * load_f32(p.w_scale[1] + n) * sx;
                 if (p.gate != nullptr) {
                     p.gate[m * p.ld_gate + n] = __float2bfloat16_rn(y);
                     p.up[m * p.ld_up + n] = __float2bfloat16_rn(u);

@@ -74,8 +74,7 @@ __device__ __forceinline__ uint2 int8_codes8(const uint4& v, const RowScale& r) 
 // NV 16-byte pieces per thread.  CTA_ROW: one row per CTA, else one per warp.  NV == 0: a row of any length, read twice.
 template <int NV, bool CTA_ROW>
 __global__ void __launch_bounds__(kInt8Threads)
-quantize_int8_kernel(const __nv_bfloat16* __restrict__ x, long long rows, int k, long long ldx, int8_t* __restrict__ values,
-                     long long ldv, float* __restrict__ scales) {
+quantize_int8_kernel(const __nv_bfloat16* x, long long rows, int k, long long ldx, int8_t* values, long long ldv, float* scales) {
     constexpr int kRowThreads = CTA_ROW ? kInt8Threads : 32;
     constexpr int kKeep = NV > 0 ? NV : 1;
     __shared__ uint32_t warp_top[kInt8Threads / 32];
@@ -95,12 +94,12 @@ quantize_int8_kernel(const __nv_bfloat16* __restrict__ x, long long rows, int k,
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int i = i0 + j * kRowThreads;
-            v[j] = (i < pieces) ? __ldcs(src + i) : make_uint4(0u, 0u, 0u, 0u);
+            v[j] = load_16<true>(src + i, i < pieces);
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) top = max_magnitude(top, v[j]);
     } else {
-        for (int i = i0; i < pieces; i += kRowThreads) top = max_magnitude(top, __ldg(src + i));
+        for (int i = i0; i < pieces; i += kRowThreads) top = max_magnitude(top, load_16(src + i));
     }
     top = max(top >> 16, top & 0xffffu);
     top = __reduce_max_sync(0xffffffffu, top);
@@ -119,7 +118,7 @@ quantize_int8_kernel(const __nv_bfloat16* __restrict__ x, long long rows, int k,
             if (i < pieces) dst[i] = int8_codes8(v[j], r);
         }
     } else {
-        for (int i = i0; i < pieces; i += kRowThreads) dst[i] = int8_codes8(__ldg(src + i), r);
+        for (int i = i0; i < pieces; i += kRowThreads) dst[i] = int8_codes8(load_16(src + i), r);
     }
 }
 

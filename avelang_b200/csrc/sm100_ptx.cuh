@@ -37,6 +37,37 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// Loads of what an earlier kernel in the stream may have written.  A kernel launched with programmatic stream serialisation is
+// resident while its predecessor still writes, so to it no such memory is read-only: no ld.global.nc, which is what __ldg and
+// const __restrict__ parameters come to.  Volatile, so that none moves above pdl_wait_prior_grid().
+// 16 bytes, or zeros where `in` is false; ONCE: not wanted again soon.
+template <bool ONCE = false>
+__device__ __forceinline__ uint4 load_16(const void* at, bool in = true) {
+    uint4 v;
+    if constexpr (ONCE) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+            "@p ld.global.cs.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+            : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(at), "r"(static_cast<uint32_t>(in)) : "memory");
+    } else {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+            "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+            : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(at), "r"(static_cast<uint32_t>(in)) : "memory");
+    }
+    return v;
+}
+__device__ __forceinline__ uint32_t load_32(const void* at) {
+    uint32_t v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float load_f32(const float* at) { return __uint_as_float(load_32(at)); }
+__device__ __forceinline__ float4 load_f32x4(const float* at) {
+    const uint4 v = load_16(at);
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+
 // One lane of the (fully active) warp gets true.
 __device__ __forceinline__ bool elect_one_sync() {
     uint32_t pred;
