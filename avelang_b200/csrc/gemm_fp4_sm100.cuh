@@ -149,7 +149,7 @@ __device__ __forceinline__ void convert_bias_act(uint32_t (&packed)[NCOLS], floa
         float b0 = 0.0f, b1 = 0.0f;
         const int col = col0 + 2 * i;
         if (bias != nullptr && col < n) {
-            const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(bias + col));
+            const uint32_t w = load_32(bias + col);
             b0 = __uint_as_float(w << 16);
             b1 = __uint_as_float(w & 0xffff0000u);
         }
@@ -457,11 +457,11 @@ gemm_fp4_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         // everything this role reads (tensor scales, bias) or writes may be touched by the previous kernel
         if (p.pdl) pdl_wait_prior_grid();
         float alpha = 1.0f;
-        if (p.a_gs) alpha *= __ldg(p.a_gs);
-        if (p.b_gs) alpha *= __ldg(p.b_gs);
+        if (p.a_gs) alpha *= load_f32(p.a_gs);
+        if (p.b_gs) alpha *= load_f32(p.b_gs);
         // constants of the quantising epilogue (the divisions a / 6 / gs are done with reciprocals, see quantize_block)
         float q_gs = 1.0f;
-        if (EPI == kEpiQuant && SF_VEC == 16 && p.q_gs != nullptr) q_gs = __ldg(p.q_gs);
+        if (EPI == kEpiQuant && SF_VEC == 16 && p.q_gs != nullptr) q_gs = load_f32(p.q_gs);
         const bool q_gs_plain = divisor_is_plain(q_gs);
         const float q_gs_recip = __frcp_rn(q_gs);
         const float sixth = __frcp_rn(6.0f);

@@ -18,6 +18,8 @@
 
 #include <cstdint>
 
+#include "sm100_ptx.cuh"
+
 namespace avefp4 {
 
 constexpr int kFmtNvfp4 = 0;
@@ -368,8 +370,8 @@ __device__ __forceinline__ void quantize_items_nvfp4_tab(const uint32_t (&rw)[NI
 // two whole NVFP4 blocks or one MXFP4 block (so a block maximum needs no exchange between lanes),
 // one 128-bit store of 32 nibbles and one 16-bit / 8-bit scale store.
 template <int FMT, bool TILED>
-__device__ __forceinline__ void quantize_rows(const __nv_bfloat16* __restrict__ x, long long rows, long long k, long long ldx,
-                                              float gs, uint8_t* __restrict__ packed, uint8_t* __restrict__ sf,
+__device__ __forceinline__ void quantize_rows(const __nv_bfloat16* x, long long rows, long long k, long long ldx,
+                                              float gs, uint8_t* packed, uint8_t* sf,
                                               long long warp_global, long long warps_total, const Nvfp4Tables* tab = nullptr) {
     constexpr int BLK = (FMT == kFmtNvfp4) ? 16 : 32;
     const int lane = threadIdx.x & 31;
@@ -401,7 +403,7 @@ __device__ __forceinline__ void quantize_rows(const __nv_bfloat16* __restrict__ 
             const uint4* src = reinterpret_cast<const uint4*>(x + rr * ldx + e);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint4 v = __ldg(src + i);
+                const uint4 v = load_16(src + i);
                 dst[4 * i] = v.x; dst[4 * i + 1] = v.y; dst[4 * i + 2] = v.z; dst[4 * i + 3] = v.w;
             }
         }
@@ -458,9 +460,8 @@ constexpr int kQuantThreads = 128;
 
 template <int FMT, bool TILED>
 __global__ void __launch_bounds__(kQuantThreads)
-quantize_fp4_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long long k, long long ldx,
-                    const unsigned int* __restrict__ amax_bits, float* __restrict__ gs_io,
-                    uint8_t* __restrict__ packed, uint8_t* __restrict__ sf) {
+quantize_fp4_kernel(const __nv_bfloat16* x, long long rows, long long k, long long ldx,
+                    const unsigned int* amax_bits, float* gs_io, uint8_t* packed, uint8_t* sf) {
     // a kernel queued behind this one with programmatic stream serialisation may start its prologue now
     // (it still waits for this grid to finish before it reads what is written here); this kernel is launched
     // the same way and waits for its own predecessor before it touches memory
@@ -471,11 +472,11 @@ quantize_fp4_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long lo
     float gs = 1.0f;
     if (FMT == kFmtNvfp4) {
         if (amax_bits != nullptr) {
-            const float amax = __uint_as_float(*amax_bits);
+            const float amax = __uint_as_float(load_32(amax_bits));
             gs = (amax == 0.0f) ? 1.0f : __fdiv_rn(amax, 2688.0f);
             if (blockIdx.x == 0 && threadIdx.x == 0) *gs_io = gs;
         } else {
-            gs = *gs_io;
+            gs = load_f32(gs_io);
         }
     }
     if constexpr (FMT == kFmtNvfp4) {
@@ -496,8 +497,8 @@ constexpr int kFusedThreads = 512;
 
 template <bool TILED>
 __global__ void __cluster_dims__(kFusedClusterCtas, 1, 1) __launch_bounds__(kFusedThreads)
-quantize_nvfp4_fused_small_kernel(const __nv_bfloat16* __restrict__ x, long long rows, long long k, long long ldx,
-                                  float* __restrict__ gs_out, uint8_t* __restrict__ packed, uint8_t* __restrict__ sf) {
+quantize_nvfp4_fused_small_kernel(const __nv_bfloat16* x, long long rows, long long k, long long ldx,
+                                  float* gs_out, uint8_t* packed, uint8_t* sf) {
     __shared__ float s_warp[kFusedThreads / 32];
     __shared__ float s_cta;
     // Launched with programmatic stream serialisation: this grid may be scheduled while the previous kernel in
@@ -520,7 +521,7 @@ quantize_nvfp4_fused_small_kernel(const __nv_bfloat16* __restrict__ x, long long
             v[u] = make_uint4(0, 0, 0, 0);
             if (g < total) {
                 const long long r = g / groups_per_row;
-                v[u] = __ldg(reinterpret_cast<const uint4*>(x + r * ldx + (g - r * groups_per_row) * 8));
+                v[u] = load_16(x + r * ldx + (g - r * groups_per_row) * 8);
             }
         }
 #pragma unroll
@@ -575,8 +576,8 @@ constexpr long long kDecodeQuantBlocks = static_cast<long long>(kFusedClusterCta
 
 template <bool TILED>
 __global__ void __cluster_dims__(kFusedClusterCtas, 1, 1) __launch_bounds__(kDecodeQuantThreads, 1)
-quantize_nvfp4_decode_kernel(const __nv_bfloat16* __restrict__ x, int rows, int k, long long ldx,
-                             float* __restrict__ gs_out, uint8_t* __restrict__ packed, uint8_t* __restrict__ sf) {
+quantize_nvfp4_decode_kernel(const __nv_bfloat16* x, int rows, int k, long long ldx,
+                             float* gs_out, uint8_t* packed, uint8_t* sf) {
     __shared__ uint32_t s_warp[kDecodeQuantThreads / 32];
     __shared__ uint32_t s_all[kFusedClusterCtas];     // every CTA's maximum, written here by the CTAs themselves
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -594,7 +595,7 @@ quantize_nvfp4_decode_kernel(const __nv_bfloat16* __restrict__ x, int rows, int 
     uint32_t rw[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
     if (mine) {
         const uint4* src = reinterpret_cast<const uint4*>(x + static_cast<long long>(row) * ldx + cb * 16);
-        const uint4 v0 = __ldg(src), v1 = __ldg(src + 1);
+        const uint4 v0 = load_16(src), v1 = load_16(src + 1);
         rw[0] = v0.x; rw[1] = v0.y; rw[2] = v0.z; rw[3] = v0.w;
         rw[4] = v1.x; rw[5] = v1.y; rw[6] = v1.z; rw[7] = v1.w;
     }
