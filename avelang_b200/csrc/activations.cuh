@@ -27,7 +27,18 @@ __device__ __forceinline__ float normal_tail(float ax) {
     return 0.5f * p * t * __expf(-0.5f * ax * ax);
 }
 
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 1 / (1 + e^-x) with numerator and denominator taken 2^-8 times: __fdividef gives 0 for a divisor beyond 2^126, which 1 + e^-x passes
+// at x = -87.3, where silu is still -1e-36.  So every silu in the normal range of fp32 (to x = -91.9) keeps its relative error; below, 0.
+__device__ __forceinline__ float sigmoid(float x) {
+    constexpr float kLog2E = 1.44269504088896341f, kPart = 0.00390625f;
+    return __fdividef(kPart, kPart + exp2_approx(fmaf(x, -kLog2E, -8.0f)));
+}
 
 // twice the argument of the tanh form: 0.5 (1 + tanh u) = sigmoid(2u)
 __device__ __forceinline__ float gelu_tanh_arg(float x) { return 1.59576912160573071f * fmaf(0.044715f * x * x, x, x); }
@@ -40,9 +51,9 @@ __device__ __forceinline__ float act_value(float x) {
         const float tail = normal_tail(fabsf(x));
         return x < 0.0f ? x * tail : x * (1.0f - tail);
     } else if constexpr (ACT == AVE_FP4_ACT_GELU_TANH) {
-        return __fdividef(x, 1.0f + __expf(-gelu_tanh_arg(x)));
+        return x * sigmoid(gelu_tanh_arg(x));
     } else if constexpr (ACT == AVE_FP4_ACT_SILU) {
-        return __fdividef(x, 1.0f + __expf(-x));
+        return x * sigmoid(x);
     } else {
         return x;
     }
