@@ -48,3 +48,41 @@ def test_beyond_two_to_the_31_elements(cuda_device):
         D.check(dwg[cols], want[1], f"{cols}")
         D.check(dwu[cols], want[2], f"{cols}")
     ave.check_device_status(cuda_device)
+
+
+def test_relu_against_differences(cuda_device):
+    """Gates are odd multiples of 1/8: exact in bf16 and never at relu's kink, so that every difference says something."""
+    m, f, h = 20, 24, 16
+    g = torch.Generator(device=cuda_device).manual_seed(0)
+    x = (torch.randint(-1, 2, (m, h), generator=g, device=cuda_device) / 4).to(torch.bfloat16)
+    wg, wu = ((torch.randint(-1, 2, (f, h), generator=g, device=cuda_device)).to(torch.bfloat16) for _ in range(2))
+    x[:, 0], wg[:, 0] = 0.125, 1.0
+    dout = _randn(cuda_device, m, f, 4)
+    _, gate, up = ave.gemm_gated_transposed_b(x, wg, wu, activation="relu", save=True)
+    assert torch.equal(gate.double(), x.double() @ wg.double().T) and gate.abs().min() >= 0.125
+    assert (gate > 0).any() and (gate < 0).any()
+    got = ave.gemm_gated_backward(dout, x, wg, wu, gate, up, activation="relu")
+    want = G.gated_backward(dout, x, wg, wu, gate, up, "relu")
+    args = [x.double(), wg.double(), wu.double()]
+    step = 2.0 ** -10      # exact, and times a weight of 1 nowhere near 1/8
+
+    def loss(*a):
+        return (dout.double() * D.act(a[0] @ a[1].T, "relu") * (a[0] @ a[2].T)).sum().item()
+
+    compared = 0
+    for which in range(3):
+        for i, j in ((0, 0), (3, 5), (19, 15), (11, 2)):
+            plus, minus = [t.clone() for t in args], [t.clone() for t in args]
+            plus[which][i, j] += step
+            minus[which][i, j] -= step
+            # quadratic in each argument: the central difference is the derivative, up to 2^-52 of a loss of some thousand, some additions long, over the step: below 1e-9
+            slope = (loss(*plus) - loss(*minus)) / (2 * step)
+            exact = want[which][0][i, j].item()
+            # the inner gradients' own rounding is in `want` and not in the loss
+            inner = {0: lambda: D.BF16 * ((dout.double() * up.double()).abs() @ args[1].abs() + (dout.double() * gate.double()).abs() @ args[2].abs()),
+                     1: lambda: D.BF16 * ((dout.double() * up.double()).abs().T @ args[0].abs()),
+                     2: lambda: D.BF16 * ((dout.double() * gate.double()).abs().T @ args[0].abs())}[which]()[i, j].item()
+            assert abs(exact - slope) <= inner + 1e-8 * (1 + abs(slope))
+            assert abs(got[which][i, j].item() - slope) <= want[which][1][i, j].item() + inner + 1e-8 * (1 + abs(slope))
+            compared += 1
+    assert compared == 12
