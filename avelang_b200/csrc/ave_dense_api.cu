@@ -400,24 +400,22 @@ PairPlan plan_pair(int sms, int64_t m0, int64_t n0, int64_t k0, int segments, in
     return best;
 }
 
-// As plan_for: found once for a size and kept by each host thread.
+// As plan_for: found once for a size and kept by each host thread, those of gated blocks and of products in slots of their own.
 const PairPlan& pair_for(const HostDevice& dev, int64_t m, int64_t n, int64_t k, bool gated) {
     struct Slot {
         int64_t m, n, k;
         int sms;
-        bool gated;
         PairPlan plan;
     };
-    thread_local Slot slots[kPlanSlots] = {};
-    Slot& slot = slots[plan_slot(m, n, k)];
-    if (slot.m != m || slot.n != n || slot.k != k || slot.sms != dev.sm_count || slot.gated != gated) {
+    thread_local Slot slots[2][kPlanSlots] = {};
+    Slot& slot = slots[gated ? 1 : 0][plan_slot(m, n, k)];
+    if (slot.m != m || slot.n != n || slot.k != k || slot.sms != dev.sm_count) {
         // gated: dX (m, k) = dG Wg + dU Wu over n, dWg and dWu (n, k) over m; else dA (m, k) over n and dB (n, k) over m
         slot.plan = plan_pair(dev.sm_count, m, k, n, gated ? 2 : 1, n, k, m, gated ? 2 : 1);
         slot.m = m;
         slot.n = n;
         slot.k = k;
         slot.sms = dev.sm_count;
-        slot.gated = gated;
     }
     return slot.plan;
 }
