@@ -440,11 +440,19 @@ int launch_sums(const HostDevice& dev, const SplitSums& sums, cudaStream_t strea
 // The streaming kernel works in units of 16 weight rows, of about a microsecond each however short K is, and takes K in steps of
 // 4 KB; the tile kernel needs a long K to fill its pipeline, and does without either.  us, streaming / tile: int8 1 x 1600 x 8192
 // 5.7 / 11.6, 1 x 4800 x 8192 11.3 / 12.4, 1 x 9600 x 8192 17.7 / 17.3, 1 x 28672 x 4096 24.2 / 23.1, 6 x 28672 x 6144 37.6 / 32.2,
-// 1 x 28672 x 8192 39.2 / 42.3, gated 1 x 28672 x 8192 72 / 77.  For 9 to 16 rows its activations do not fit L1 beside the
-// ring: 16 x 1024 x 8192 6.1 / 13.3, 16 x 4096 x 4096 8.0 / 7.7, 16 x 28672 x 8192 48.6 / 42.5.
+// 1 x 28672 x 8192 39.2 / 42.3, gated 1 x 28672 x 8192 72 / 77.  So with more than two units an SM it takes whole steps only, two of
+// them, or for one token up to four: longer activations do not stay in what the ring leaves of L1.  int8, K in bytes, 28672 weight rows:
+//   one token     8192 39.7 / 42.1, 12288 55.9 / 57.8, 16384 72.6 / 75.5, 24576 109.2 / 107.6, 28672 126.9 / 125.1
+//   eight         8192 42.8 / 42.9, 12288 60.1 / 58.3, 16384 77.8 / 76.3, 24576 112.8 / 109.1, 28672 134.1 / 126.5 (9600 rows 53.2 / 46.6)
+//   one token, a step in part    8208 49.6 / 43.7, 10240 50.5 / 49.7, 11008 52.1 / 53.0, 13824 65.8 / 64.5, 14336 71.3 / 66.1,
+//                                15360 70.8 / 71.1, 18944 86.0 / 92.8 (the most it would gain), 27648 129 / 121
+//   eight, a step in part        8208 52.7 / 44.4, 11008 57.9 / 53.7, 14336 73.4 / 66.5, 18944 99.6 / 94.1, 27648 135 / 122
+// bf16 gated 14336, K in bytes: one token 8192 38.8 / 40.9, 16384 72.0 / 73.6; eight 8192 40.5 / 41.0, 16384 77.4 / 74.0.
+// For 9 to 16 rows its activations do not fit L1 beside the ring: 16 x 1024 x 8192 6.1 / 13.3, 16 x 4096 x 4096 8.0 / 7.7,
+// 16 x 28672 x 8192 48.6 / 42.5.
 bool stream_rows(const HostDevice& dev, int64_t m, int64_t weight_rows, int64_t k_bytes) {
     const int64_t units = (weight_rows + 15) / 16;
-    if (m <= 8) return units <= 2 * dev.sm_count || (k_bytes >= 8192 && k_bytes % 4096 == 0);
+    if (m <= 8) return units <= 2 * dev.sm_count || k_bytes == 8192 || (k_bytes > 8192 && k_bytes % 4096 == 0 && m * k_bytes <= 16384);
     return m <= 16 && units <= dev.sm_count;
 }
 
