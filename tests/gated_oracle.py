@@ -27,12 +27,18 @@ def gated_backward(dout, x, wg, wu, gate, up, activation):
     x, wg, wu = x.double(), wg.double(), wu.double()
     (dg, eg), (du, eu) = inner_gradients(dout, gate, up, activation)
     m, f = dg.shape
-    dx, sx, ex = dg @ wg + du @ wu, dg.abs() @ wg.abs() + du.abs() @ wu.abs(), eg @ wg.abs() + eu @ wu.abs()
-    results = [(dx, D.BF16 * dx.abs() + D.sum_bound(2 * f) * sx + ex)]
+    dx = dg @ wg + du @ wu
+    results = [(dx, _bound(dx, D.sum_bound(2 * f) * (dg.abs() @ wg.abs() + du.abs() @ wu.abs()) + eg @ wg.abs() + eu @ wu.abs()))]
     for inner, slack in ((dg, eg), (du, eu)):
         dw = inner.T @ x
-        results.append((dw, D.BF16 * dw.abs() + D.sum_bound(m) * (inner.abs().T @ x.abs()) + slack.T @ x.abs()))
+        results.append((dw, _bound(dw, D.sum_bound(m) * (inner.abs().T @ x.abs()) + slack.T @ x.abs())))
     return results
+
+
+def _bound(value, off):
+    """Of a sum that is off by at most `off` before it is rounded: the rounding is relative to |value| + off, which after an inner value
+    that went the other way may be many times |value|."""
+    return off + D.BF16 * (value.abs() + off)
 
 
 def check(got, want, what=""):
