@@ -1,4 +1,5 @@
-// Activations of the integer, gated and gradient kernels: values and slopes in fp32.
+// Activations of the integer, gated and gradient kernels: values and slopes in fp32.  (The FP4 tiles' epilogue keeps the forms in
+// gemm_fp4_sm100.cuh, with a bound on gelu's absolute error; there relu of a NaN is 0, here it is a NaN.)
 //
 // erf enters through erfcx(z) = exp(z^2) erfc(z), z >= 0, as t P(t) with t = 1 / (1 + 0.6 z) and a degree-7 P fitted
 // to the smallest relative error over 0 <= z <= 13.5 (3.5e-7 as a polynomial, 4.4e-7 evaluated in fp32).  A bound on the

@@ -336,7 +336,7 @@ struct PlanChoices {
 // Both products in turn, each planned alone / both together, us: gated backward 1003x2744x1048 41.5 / 36.9, 1144x1040x216 21.6 / 17.7,
 // product gradients 744x7384x248 21.5 / 16.0, 6480x584x216 19.8 / 13.7; the worst of 220 sizes 880x1800x160 11.1 / 12.3, on average
 // 1.7 % less.  Left as planned alone: what memory bounds for half of the time or more (8x11504x2264 31 / 43, for all SMs share that
-// however the tiles lie), and what would gain less than 5 % by the estimate (2048x4096x1024 69 / 73).
+// however the tiles lie), and what would gain less than 5 % by the estimate (gated backward 2048x4096x1024 69 / 73).
 // Where memory bounds the products of a few rows, one of which reads the weights and the other writes their gradients, they run
 // beside each other, each on half of the SMs: copying goes at 6.2 TB/s, writing alone at 4.  The second's CTAs are single ones, for
 // pairs find no two free neighbours, and take 85 % of its tiles before the first is done.  One after the other / beside each other,

@@ -495,9 +495,10 @@ gemm_dense_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
                         // 32 rows x up to 32 columns through a transpose in shared memory, so that a row's part of the result is
                         // stored by neighbouring lanes.  Or directly, in whole 32-byte sectors: at the tensor pipe's full rate its
                         // operands take all of shared memory's 128 bytes a clock, and the transpose slows it down.  int8 with gelu_tanh and
-                        // bias, transposed / direct, us: 2048 x 8192 x 1024 37.2 / 35.0, 8192 x 8192 x 512 76 / 71, 8192^3 the same; gated
-                        // int8 4096 x 8192 x 1024 56.5 / 55.8, gated bf16 4096 x 16384 x 4096 805 / 808, and gradients of 512 x 8192 x 8192,
-                        // bound by writing, 110 / 117, so the others keep to the transpose.
+                        // bias, transposed / direct, us: 2048 x 8192 x 1024 25.9 / 24.3 (at 1.9 GHz), 8192 x 8192 x 512 76 / 72, 8192 x 8192 x 1024
+                        // 82.7 / 78.9 (63.3 / 65.1 without an activation), 8192^3 the same; gated int8 4096 x 8192 x 1024 56.5 / 55.8, gated
+                        // bf16 4096 x 16384 x 4096 805 / 808, and gradients of 512 x 8192 x 8192, bound by writing, 110 / 117, so the
+                        // others keep to the transpose.
 #pragma unroll 1
                         for (int c = c0; c < c1; c += 16) {
                             uint32_t v[16], u[16], w[8];
