@@ -341,8 +341,8 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_co
         // previous kernel in the stream
         if (p.pdl) pdl_wait_prior_grid();
         float alpha = 1.0f;
-        if (p.x_gs) alpha *= __ldcg(p.x_gs);
-        if (p.w_gs) alpha *= __ldcg(p.w_gs);
+        if (p.x_gs) alpha *= load_f32(p.x_gs);
+        if (p.w_gs) alpha *= load_f32(p.w_gs);
         int seg = 0;
         bool ok = true;
         long long u = u_begin;
@@ -413,7 +413,7 @@ gemm_fp4_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_co
                     for (int c = c0; c <= c1; ++c) {
                         const float* src = p.partials + (static_cast<size_t>(c) * 2 + (c == c0 ? 1 : 0)) * (MP * 128);
 #pragma unroll
-                        for (int m = 0; m < MP; ++m) v[m] = __float_as_uint(__uint_as_float(v[m]) + __ldcg(src + m * 128 + n_local));
+                        for (int m = 0; m < MP; ++m) v[m] = __float_as_uint(__uint_as_float(v[m]) + load_f32_l2(src + m * 128 + n_local));
                     }
                     final_here = true;
                 }

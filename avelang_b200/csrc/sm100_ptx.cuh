@@ -62,6 +62,12 @@ __device__ __forceinline__ uint32_t load_32(const void* at) {
     asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
     return v;
 }
+// past L1: what another CTA of this grid has written
+__device__ __forceinline__ float load_f32_l2(const float* at) {
+    float v;
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(at) : "memory");
+    return v;
+}
 __device__ __forceinline__ float load_f32(const float* at) { return __uint_as_float(load_32(at)); }
 __device__ __forceinline__ float4 load_f32x4(const float* at) {
     const uint4 v = load_16(at);

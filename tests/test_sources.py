@@ -44,7 +44,7 @@ def test_no_non_coherent_loads_beside_a_running_predecessor(name):
     code = _code(name)
     for kernel in ORDERED:
         code = _without(code, kernel)
-    found = re.findall(r"__ld(?:g|cs|ca|lu|cv)\s*\(|ld\.global\.nc", code)
+    found = re.findall(r"__ld(?:g|cs|cg|ca|lu|cv)\s*\(|ld\.global\.nc", code)
     assert not found, found
     for signature in re.findall(r"__global__[^{;]*", code):
         assert "__restrict__" not in signature, signature
